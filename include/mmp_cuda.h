@@ -111,8 +111,8 @@ int mmp_synchronize(void);
 /* Synchronise, then read and clear the device-side error word that kernels
  * set instead of hanging or writing out of bounds: 0 = no error, 2 = scan
  * look-back wait ran out, 3 = GEMM pipeline wait ran out, 4 = sort scatter
- * offset out of range, 5 = gather / scatter / compaction offset out of
- * range, 6 = the self-test wait ran out (mmp_selftest_bounded_wait),
+ * offset out of range, 5 = gather / scatter / compaction offset or
+ * embedding id out of range, 6 = the self-test wait ran out (mmp_selftest_bounded_wait),
  * 8 = a peer's flag did not arrive in mmp_reduce_allranks,
  * mmp_scan_allranks or mmp_allreduce_sum_peer. */
 int mmp_check_device_error(int *code);
@@ -243,6 +243,57 @@ int mmp_scatter(int dtype, void *dst, int64_t limit, const int64_t *offsets,
  * flatnonzero). */
 int mmp_compact_indices(const void *mask, const int64_t *incl, int64_t n,
                         int64_t count, int64_t *out);
+
+/* ---- operators of sequence models.  The reference has none of them; each
+ * extends one of its own (cumsum / cumprod, reductions.py:661-705; take,
+ * indexing.py:24-60; sum, reductions.py:74-113).  Floating dtypes only;
+ * states, sums and norms are held in float32, or float64 for float64
+ * arrays (the norm: float64 always), and outputs rounded once. */
+
+/* First-order recurrence h_t = f_t h_{t-1} + u_t along the middle axis of
+ * (outer, steps, inner): f = a, u = x, or with `gated` f = sigmoid(a),
+ * u = (1 - f) x.  a, x and h are addressed as base + o * so + t * st + i
+ * elements (strides of any sign, 0 for inputs).  h0 (NULL: zeros) and
+ * `state` (NULL, or the state after the last step; may be h0) are
+ * contiguous (outer, inner) in float32 (float64 for float64 arrays).
+ * h may be a or x itself; any other overlap of h with an input is not
+ * checked and gives wrong results. */
+int mmp_recurrence(int dtype, int gated, int64_t outer, int64_t steps, int64_t inner,
+                   const void *a, int64_t a_so, int64_t a_st, const void *x, int64_t x_so,
+                   int64_t x_st, const void *h0, void *h, int64_t h_so, int64_t h_st, void *state);
+/* Its gradient, from h and grad = dL/dh: grad_a, grad_x and (NULL: not
+ * wanted) grad_h0; grad_state (NULL: zeros) is dL/dstate.  x is read with
+ * `gated` only.  grad_a / grad_x may each be one of a, x, grad themselves,
+ * grad_h0 may be grad_state; no other overlap. */
+int mmp_recurrence_grad(int dtype, int gated, int64_t outer, int64_t steps, int64_t inner,
+                        const void *a, int64_t a_so, int64_t a_st, const void *x, int64_t x_so,
+                        int64_t x_st, const void *h, int64_t h_so, int64_t h_st, const void *grad,
+                        int64_t g_so, int64_t g_st, const void *h0, const void *grad_state,
+                        void *grad_a, int64_t ga_so, int64_t ga_st, void *grad_x, int64_t gx_so,
+                        int64_t gx_st, void *grad_h0);
+
+/* out[n, :] = scale * weight[ids[n], :] for a (rows, width) table with rows
+ * w_stride elements apart; ids int32 or int64; out is C-contiguous.  An id
+ * outside [0, rows) gives zeros and device error 5. */
+int mmp_embedding(int dtype, const void *weight, int64_t rows, int64_t width, int64_t w_stride,
+                  int ids_dtype, const void *ids, int64_t n, double scale, void *out);
+/* grad_weight[v, :] = scale * sum of grad[n, :] over ids[n] == v, added in a
+ * fixed order (equal calls give equal bits); every row is written, rows
+ * without an id and row padding_idx (-1: none) with zeros.  grad's rows are
+ * g_stride elements apart.  An id outside [0, rows) adds nothing and sets
+ * device error 5. */
+int mmp_embedding_grad(int dtype, int ids_dtype, const void *ids, int64_t n, const void *grad,
+                       int64_t g_stride, int64_t rows, int64_t width, double scale,
+                       int64_t padding_idx, void *grad_weight);
+
+/* norm = sqrt(sum of squares of all elements of `count` contiguous arrays
+ * (sizes in elements, each with its dtype)), written to device memory as
+ * norm_dtype (float32 or float64).  With y, also y[i] = x[i] * (norm <=
+ * max_norm ? 1 : max_norm / norm), each y[i] in x[i]'s dtype and either
+ * x[i] itself or apart from every x.  dtypes, x, y and sizes are host
+ * arrays, read before the call returns. */
+int mmp_global_norm(int64_t count, const int *dtypes, const void *const *x, void *const *y,
+                    const int64_t *sizes, double max_norm, int norm_dtype, void *norm);
 
 /* ---- block-distributed arrays: partials and their merge on the device.
  * The reference is single-device (MetalBackend, _metal_backend.py:186-204);

@@ -98,6 +98,13 @@ SIGNATURES = {
     "mmp_gather": (_int, [_int, _vp, _i64, _vp, _i64, _vp]),
     "mmp_scatter": (_int, [_int, _vp, _i64, _vp, _i64, _vp]),
     "mmp_compact_indices": (_int, [_vp, _vp, _i64, _i64, _vp]),
+    "mmp_recurrence": (_int, [_int, _int, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64,
+                              _vp]),
+    "mmp_recurrence_grad": (_int, [_int, _int, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64,
+                                   _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp]),
+    "mmp_embedding": (_int, [_int, _vp, _i64, _i64, _i64, _int, _vp, _i64, ctypes.c_double, _vp]),
+    "mmp_embedding_grad": (_int, [_int, _int, _vp, _i64, _vp, _i64, _i64, _i64, ctypes.c_double, _i64, _vp]),
+    "mmp_global_norm": (_int, [_i64, _vp, _vp, _vp, _vp, ctypes.c_double, _int, _vp]),
     "mmp_reduce_partial": (_int, [_int, _int, _vp, _i64, _i64, _vp]),
     "mmp_merge_partials": (_int, [_int, _int, _vp, _int, _int, _vp, ctypes.c_double, _vp]),
     "mmp_nccl_version": (_int, [ctypes.POINTER(_int)]),
