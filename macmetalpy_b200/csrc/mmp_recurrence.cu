@@ -47,12 +47,23 @@ template <> struct RecState<double> { typedef double type; };
 // f = sigmoid(z) and 1 - f from e = exp(-|z|) in (0, 1], so that neither
 // cancels and z = +-inf gives exactly 1 and 0 (e = 0): a gate of +inf keeps
 // the state as it is, one of -inf replaces it.  A NaN goes to both.  float16
-// gates use __expf, whose error of 2 + 1.2 |z| ulp is far below theirs.
-template <class T> __device__ __forceinline__ float rec_exp(float z) { return expf(z); }
-template <> __device__ __forceinline__ float rec_exp<__half>(float z) { return __expf(z); }
+// gates take ex2.approx and rcp.approx (relative errors 2^-22.5 + |z| 2^-24 and
+// 2^-23, far below the gates' own rounding of 2^-11): the kernel issues some
+// 20 instructions an element, and expf and the division would add as many.
+__device__ __forceinline__ float rec_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rec_rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 template <class T> __device__ __forceinline__ void rec_gate(float z, float &f, float &rest) {
-  const float e = rec_exp<T>(-fabsf(z));
-  const float r = __fdividef(1.0f, 1.0f + e);
+  constexpr bool half = sizeof(T) == 2;
+  const float e = half ? rec_ex2(fabsf(z) * -1.4426950408889634f) : expf(-fabsf(z));
+  const float r = rec_rcp(1.0f + e);
   const float q = e * r;
   f = z < 0.0f ? q : r;
   rest = z < 0.0f ? r : q;
@@ -71,12 +82,11 @@ template <class S> __device__ __forceinline__ S rec_apply(S A, S H, S s) { retur
 
 template <class T, int VEC> struct alignas(sizeof(T) * VEC) RecVec { T v[VEC]; };
 
-template <int BYTES> __device__ __forceinline__ void rec_cp_async(void *dst, const void *src) {
-  const unsigned d = (unsigned)__cvta_generic_to_shared(dst);
+template <int BYTES> __device__ __forceinline__ void rec_cp_async(unsigned dst, const void *src) {
   if (BYTES == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src) : "memory");
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
   else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(d), "l"(src), "n"(BYTES) : "memory");
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
 }
 __device__ __forceinline__ void rec_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // Waits until at most `n` of this thread's newest groups are still on the way.
@@ -92,28 +102,36 @@ struct RecArgs {
   const void *h0;
   const void *seed;  // the state before the first span: h0 / grad_state
   void *last;        // the state after the last span: state / grad_h0
-  long long groups, steps, per;  // per: groups along inner
-  int iters, stages;
+  long long groups, per;  // per: groups along inner
+  int steps, iters, stages;
+  int near;  // every step stride is below 2^31 bytes
 };
 
 constexpr int kRecWarps = 8;
 
-// Steps of one warp's span: 16 forward, 8 backward (its ring holds more
-// arrays).
-template <bool GRAD> struct RecSpan { static constexpr int value = GRAD ? 8 : 16; };
+// Steps of one warp's span, by the bytes that a lane moves a step: 32 KB of
+// ring a stage and block of 8 warps, so that two blocks of three stages fit an
+// SM.
+template <int BYTES, bool GRAD> struct RecSpan { static constexpr int value = (GRAD ? 8 : 16) / (BYTES == 8 ? 2 : 1); };
+
+template <class S> struct alignas(2 * sizeof(S)) RecMap {
+  S a, h;
+};
 
 template <class T, int VEC, bool GRAD, bool GATED, bool CLUSTER>
 __global__ void __launch_bounds__(32 * kRecWarps, 2) rec_kernel(const __grid_constant__ RecArgs g) {
   typedef typename RecState<T>::type S;
   typedef RecVec<T, VEC> V;
-  constexpr int N = RecSpan<GRAD>::value;
+  constexpr int N = RecSpan<(int)sizeof(V), GRAD>::value;
   constexpr int NA = GRAD ? (GATED ? 4 : 3) : 2;
+  constexpr int NO = GRAD ? 2 : 1;
+  constexpr int NC = 32 * VEC;            // chains of the block
   constexpr bool ASYNC = sizeof(V) >= 4;  // cp.async copies 4, 8 or 16 bytes
   extern __shared__ __align__(16) unsigned char s_ring[];
-  __shared__ S s_a[2][kRecWarps][32 * VEC], s_h[2][kRecWarps][32 * VEC];
-  __shared__ S s_ca[CLUSTER ? 2 : 1][CLUSTER ? 8 : 1][32 * VEC], s_ch[CLUSTER ? 2 : 1][CLUSTER ? 8 : 1][32 * VEC];
+  __shared__ RecMap<S> s_map[kRecWarps][NC];                         // the warps' spans
+  __shared__ RecMap<S> s_blk[CLUSTER ? 2 : 1][CLUSTER ? 8 : 1][NC];  // the cluster's blocks' spans
+  __shared__ S s_start[kRecWarps][NC], s_carry[NC];
   const int lane = threadIdx.x, w = threadIdx.y, warps = blockDim.y;
-  const int threads = 32 * warps, tid = w * 32 + lane;
   int rank = 0, ranks = 1;
   long long blk = blockIdx.x;
   if (CLUSTER) {
@@ -130,48 +148,63 @@ __global__ void __launch_bounds__(32 * kRecWarps, 2) rec_kernel(const __grid_con
   const T *in[NA];
 #pragma unroll
   for (int q = 0; q < NA; ++q) in[q] = (const T *)g.in[q].p + o * g.in[q].so + i;
-  T *out[2];
+  T *out[NO];
 #pragma unroll
-  for (int q = 0; q < (GRAD ? 2 : 1); ++q) out[q] = (T *)const_cast<void *>(g.out[q].p) + o * g.out[q].so + i;
-  V *ring = reinterpret_cast<V *>(s_ring);
-  const long long span = (long long)ranks * warps * N;  // steps of the cluster
-  const long long mine = ((long long)rank * warps + w) * N;
-  S carry[VEC];  // the state before the cluster's present span
+  for (int q = 0; q < NO; ++q) out[q] = (T *)const_cast<void *>(g.out[q].p) + o * g.out[q].so + i;
+  // this thread's slots: [stage][array][step], a row of 32 lanes each
+  V *const ring = reinterpret_cast<V *>(s_ring) + (size_t)w * g.stages * (NA * N * 32) + lane;
+  const int span = ranks * warps * N;  // steps of the cluster
+  const int mine = (rank * warps + w) * N;
+  S carry[VEC];  // the state before the present span of a block of one warp
 #pragma unroll
-  for (int v = 0; v < VEC; ++v) carry[v] = active && g.seed ? ((const S *)g.seed)[grp * VEC + v] : S(0);
+  for (int v = 0; v < VEC; ++v) {
+    carry[v] = active && g.seed ? ((const S *)g.seed)[grp * VEC + v] : S(0);
+    if (w == 0) s_carry[lane * VEC + v] = carry[v];
+  }
 
   // step k in the order of work lies at t = k forward, steps - 1 - k backward;
   // h is read one step before, so at t = 0 (where h0 stands in) not at all
   V pre[ASYNC ? 1 : NA][ASYNC ? 1 : N];
   auto issue = [&](int it) {
-    const long long k0 = it * span + mine;
-    const long long left = active ? g.steps - k0 : 0;
+    const int k0 = it * span + mine;
+    const int left = active ? g.steps - k0 : 0;
     if (left <= 0) return;
-    V *slot = ring + (size_t)(ASYNC ? it % g.stages : 0) * NA * N * threads + tid;
+    const unsigned slot = (unsigned)__cvta_generic_to_shared(ring + (ASYNC ? it % g.stages : 0) * (NA * N * 32));
+    const long long t0 = GRAD ? g.steps - 1 - k0 : k0;
+    if (left > N && g.near) {  // a whole span with one address instruction a step
+#pragma unroll
+      for (int q = 0; q < NA; ++q) {
+        const int st = (int)(GRAD ? -g.in[q].st : g.in[q].st) * (int)sizeof(T);
+        const char *p = (const char *)(in[q] + (GRAD && q == 2 ? t0 - 1 : t0) * g.in[q].st);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          const char *pj = p + (long long)st * j;
+          if constexpr (ASYNC) rec_cp_async<(int)sizeof(V)>(slot + (q * N + j) * 32 * (int)sizeof(V), pj);
+          else pre[q][j] = *reinterpret_cast<const V *>(pj);
+        }
+      }
+      return;
+    }
 #pragma unroll
     for (int q = 0; q < NA; ++q) {
       const long long st = GRAD ? -g.in[q].st : g.in[q].st;
-      const T *p = in[q] + (GRAD ? g.steps - 1 - k0 : k0) * g.in[q].st;
-      const long long n = GRAD && q == 2 ? left - 1 : left;
-      if (GRAD && q == 2) p += st;
+      const T *p = in[q] + (GRAD && q == 2 ? t0 - 1 : t0) * g.in[q].st;
+      const int n = GRAD && q == 2 ? left - 1 : left;
 #pragma unroll
       for (int j = 0; j < N; ++j) {
         if (j < n) {
-          if constexpr (ASYNC) rec_cp_async<(int)sizeof(V)>(slot + (q * N + j) * threads, p);
+          if constexpr (ASYNC) rec_cp_async<(int)sizeof(V)>(slot + (q * N + j) * 32 * (int)sizeof(V), p);
           else pre[q][j] = *reinterpret_cast<const V *>(p);
         }
         p += st;
       }
     }
   };
-  auto commit = [&]() {
-    if constexpr (ASYNC) rec_commit();
-  };
   const int ahead = ASYNC ? g.stages - 1 : 0;
   if constexpr (ASYNC) {
     for (int it = 0; it < ahead; ++it) {
       issue(it);
-      commit();
+      rec_commit();
     }
   } else {
     issue(0);
@@ -181,19 +214,18 @@ __global__ void __launch_bounds__(32 * kRecWarps, 2) rec_kernel(const __grid_con
   for (int it = 0; it < g.iters; ++it) {
     if constexpr (ASYNC) {
       if (it + ahead < g.iters) issue(it + ahead);
-      commit();
+      rec_commit();
       rec_wait(ahead);
     } else {
 #pragma unroll
       for (int q = 0; q < NA; ++q)
 #pragma unroll
-        for (int j = 0; j < N; ++j) ring[(q * N + j) * threads + tid] = pre[q][j];
+        for (int j = 0; j < N; ++j) ring[(q * N + j) * 32] = pre[q][j];
       if (it + 1 < g.iters) issue(it + 1);
     }
-    const long long k0 = it * span + mine;
-    const long long left = active ? g.steps - k0 : 0;
-    const V *slot = ring + (size_t)(ASYNC ? it % g.stages : 0) * NA * N * threads + tid;
-    auto raw = [&](int q, int j, int v) -> S { return Cvt<S, T>::f(slot[(q * N + j) * threads].v[v]); };
+    const int k0 = it * span + mine;
+    const int left = active ? g.steps - k0 : 0;
+    const V *const slot = ring + (ASYNC ? it % g.stages : 0) * (NA * N * 32);
 
     // the span's composition, from a state of zero.  Gates are evaluated once
     // and kept: f and u forward, f and 1 - f backward.
@@ -203,76 +235,71 @@ __global__ void __launch_bounds__(32 * kRecWarps, 2) rec_kernel(const __grid_con
       A[v] = S(1);
       H[v] = S(0);
     }
+    auto compose = [&](int j) {
+      const V va = slot[j * 32], vb = slot[(N + j) * 32];
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      if (j < left) {
-        const V va = slot[j * threads], vb = slot[(N + j) * threads];
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-          S f = Cvt<S, T>::f(va.v[v]), u = Cvt<S, T>::f(vb.v[v]);
-          if constexpr (GATED) {
-            S rest;
-            rec_gate<T>(f, f, rest);
-            F[j][v] = f;
-            U[j][v] = GRAD ? rest : rest * u;
-            if (!GRAD) u = U[j][v];
-          }
-          H[v] = GRAD ? f * (u + H[v]) : fma(f, H[v], u);
-          A[v] *= f;
+      for (int v = 0; v < VEC; ++v) {
+        S f = Cvt<S, T>::f(va.v[v]), u = Cvt<S, T>::f(vb.v[v]);
+        if constexpr (GATED) {
+          S rest;
+          rec_gate<T>(f, f, rest);
+          F[j][v] = f;
+          U[j][v] = GRAD ? rest : rest * u;
+          if (!GRAD) u = U[j][v];
         }
+        H[v] = GRAD ? f * (u + H[v]) : fma(f, H[v], u);
+        A[v] *= f;
       }
+    };
+    if (left >= N) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) compose(j);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (j < left) compose(j);
     }
 
-    // join the block's warps, then the cluster's blocks
-    const int par = it & 1;
+    // join the block's warps, then the cluster's blocks: one thread a chain
     S s[VEC];
     if (warps > 1 || CLUSTER) {
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        s_a[par][w][lane * VEC + v] = A[v];
-        s_h[par][w][lane * VEC + v] = H[v];
-      }
+      for (int v = 0; v < VEC; ++v) s_map[w][lane * VEC + v] = RecMap<S>{A[v], H[v]};
       __syncthreads();
+      const int tid = w * 32 + lane, par = it & 1;
       if (CLUSTER) {
-        // this block's composition to every block of the cluster, one warp a block
-        for (int r = w; r < ranks; r += warps) {
-          S *pa = cg::this_cluster().map_shared_rank(&s_ca[par][rank][0], r);
-          S *ph = cg::this_cluster().map_shared_rank(&s_ch[par][rank][0], r);
-#pragma unroll
-          for (int v = 0; v < VEC; ++v) {
-            S a = S(1), h = S(0);
-            for (int b = 0; b < warps; ++b) {
-              const S ab = s_a[par][b][lane * VEC + v];
-              h = rec_apply(ab, s_h[par][b][lane * VEC + v], h);
-              a *= ab;
-            }
-            pa[lane * VEC + v] = a;
-            ph[lane * VEC + v] = h;
+        for (int c = tid; c < NC; c += 32 * warps) {
+          RecMap<S> m = s_map[0][c];
+          for (int b = 1; b < warps; ++b) {
+            const RecMap<S> n = s_map[b][c];
+            m.h = rec_apply(n.a, n.h, m.h);
+            m.a *= n.a;
           }
+          for (int r = 0; r < ranks; ++r) *cg::this_cluster().map_shared_rank(&s_blk[par][rank][c], r) = m;
         }
         asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
       }
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        S c = carry[v];
+      for (int c = tid; c < NC; c += 32 * warps) {
+        S st = s_carry[c];
         if (CLUSTER) {
-          S start = c;
+          S at = st;
           for (int r = 0; r < ranks; ++r) {
-            if (r == rank) start = c;
-            c = rec_apply(s_ca[par][r][lane * VEC + v], s_ch[par][r][lane * VEC + v], c);
+            if (r == rank) at = st;
+            st = rec_apply(s_blk[par][r][c].a, s_blk[par][r][c].h, st);
           }
-          carry[v] = c;
-          c = start;
+          s_carry[c] = st;
+          st = at;
         }
-        s[v] = c;
         for (int b = 0; b < warps; ++b) {
-          if (b == w) s[v] = c;
-          if (b >= w && CLUSTER) break;
-          c = rec_apply(s_a[par][b][lane * VEC + v], s_h[par][b][lane * VEC + v], c);
+          s_start[b][c] = st;
+          st = rec_apply(s_map[b][c].a, s_map[b][c].h, st);
         }
-        if (!CLUSTER) carry[v] = c;
+        if (!CLUSTER) s_carry[c] = st;
       }
+      __syncthreads();
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) s[v] = s_start[w][lane * VEC + v];
     } else {
 #pragma unroll
       for (int v = 0; v < VEC; ++v) {
@@ -282,44 +309,65 @@ __global__ void __launch_bounds__(32 * kRecWarps, 2) rec_kernel(const __grid_con
     }
 
     // the span's steps again, from the state before it
-    T *po[2];
+    auto replay = [&](int j, bool first, V &r0, V &r1) {
+      V va, vb, vh, vx;
+      if (GRAD || !GATED) vb = slot[(N + j) * 32];
+      if (!GATED) va = slot[j * 32];
+      if (GRAD && !first) vh = slot[(2 * N + j) * 32];
+      if (GRAD && GATED) vx = slot[((NA - 1) * N + j) * 32];
 #pragma unroll
-    for (int q = 0; q < (GRAD ? 2 : 1); ++q) po[q] = out[q] + (GRAD ? g.steps - 1 - k0 : k0) * g.out[q].st;
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      if (j < left) {
-        V r0, r1;
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-          const S f = GATED ? F[GATED ? j : 0][v] : raw(0, j, v);
-          if (!GRAD) {
-            s[v] = fma(f, s[v], GATED ? U[GATED ? j : 0][v] : raw(1, j, v));
-            r0.v[v] = Cvt<T, S>::f(s[v]);
+      for (int v = 0; v < VEC; ++v) {
+        const S f = GATED ? F[GATED ? j : 0][v] : Cvt<S, T>::f(va.v[v]);
+        if (!GRAD) {
+          s[v] = fma(f, s[v], GATED ? U[GATED ? j : 0][v] : Cvt<S, T>::f(vb.v[v]));
+          r0.v[v] = Cvt<T, S>::f(s[v]);
+        } else {
+          const S gt = Cvt<S, T>::f(vb.v[v]) + s[v];
+          const S hp = !first ? Cvt<S, T>::f(vh.v[v]) : g.h0 ? ((const S *)g.h0)[grp * VEC + v] : S(0);
+          if constexpr (GATED) {
+            const S rest = U[j][v];
+            r0.v[v] = Cvt<T, S>::f(gt * (hp - Cvt<S, T>::f(vx.v[v])) * (f * rest));
+            r1.v[v] = Cvt<T, S>::f(gt * rest);
           } else {
-            const S gt = raw(1, j, v) + s[v];
-            S hp = S(0);
-            if (j + 1 < left) hp = raw(2, j, v);
-            else if (g.h0) hp = ((const S *)g.h0)[grp * VEC + v];
-            if constexpr (GATED) {
-              const S rest = U[j][v];
-              r0.v[v] = Cvt<T, S>::f(gt * (hp - raw(3, j, v)) * (f * rest));
-              r1.v[v] = Cvt<T, S>::f(gt * rest);
-            } else {
-              r0.v[v] = Cvt<T, S>::f(gt * hp);
-              r1.v[v] = Cvt<T, S>::f(gt);
-            }
-            s[v] = f * gt;
+            r0.v[v] = Cvt<T, S>::f(gt * hp);
+            r1.v[v] = Cvt<T, S>::f(gt);
           }
-        }
-        *reinterpret_cast<V *>(po[0]) = r0;
-        if (GRAD) *reinterpret_cast<V *>(po[1]) = r1;
-        if (k0 + j + 1 == g.steps && g.last) {
-#pragma unroll
-          for (int v = 0; v < VEC; ++v) ((S *)g.last)[grp * VEC + v] = s[v];
+          s[v] = f * gt;
         }
       }
-      po[0] += GRAD ? -g.out[0].st : g.out[0].st;
-      if (GRAD) po[1] -= g.out[1].st;
+    };
+    const long long t0 = GRAD ? g.steps - 1 - k0 : k0;
+    if (left > N && g.near) {  // whole, and not the last span
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        V r[2];
+        replay(j, false, r[0], r[1]);
+#pragma unroll
+        for (int q = 0; q < NO; ++q) {
+          const int st = (int)(GRAD ? -g.out[q].st : g.out[q].st) * (int)sizeof(T);
+          *reinterpret_cast<V *>((char *)(out[q] + t0 * g.out[q].st) + (long long)st * j) = r[q];
+        }
+      }
+    } else if (left > 0) {
+      T *po[NO];
+#pragma unroll
+      for (int q = 0; q < NO; ++q) po[q] = out[q] + t0 * g.out[q].st;
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        if (j < left) {
+          V r[2];
+          replay(j, GRAD && j + 1 == left, r[0], r[1]);
+#pragma unroll
+          for (int q = 0; q < NO; ++q) {
+            *reinterpret_cast<V *>(po[q]) = r[q];
+            po[q] += GRAD ? -g.out[q].st : g.out[q].st;
+          }
+        }
+      }
+      if (left <= N && g.last) {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) ((S *)g.last)[grp * VEC + v] = s[v];
+      }
     }
   }
   if (g.steps == 0 && g.last && active && w == 0) {
@@ -342,7 +390,7 @@ int rec_sizes(const char *what, int dtype, int64_t outer, int64_t steps, int64_t
     return mmp::set_error(MMP_E_ARG, std::string(what) + ": needs a floating dtype");
   if (inner && outer > (INT64_C(1) << 32) / inner)
     return mmp::set_error(MMP_E_ARG, std::string(what) + ": more than 2^32 chains");
-  if (steps > INT32_MAX) return mmp::set_error(MMP_E_ARG, std::string(what) + ": more than 2^31 - 1 steps");
+  if (steps > INT64_C(1) << 30) return mmp::set_error(MMP_E_ARG, std::string(what) + ": more than 2^30 steps");
   return MMP_OK;
 }
 
@@ -370,14 +418,17 @@ int rec_launch(const RecArgs &g, unsigned blocks, int warps, int ranks, size_t s
 
 template <class T, int VEC, bool GRAD, bool GATED>
 int rec_run(RecArgs g, long long chains, long long inner) {
-  constexpr int N = mmpd::RecSpan<GRAD>::value;
+  constexpr int N = mmpd::RecSpan<(int)sizeof(T) * VEC, GRAD>::value;
   constexpr int NA = GRAD ? (GATED ? 4 : 3) : 2;
   g.groups = chains / VEC;
   g.per = inner / VEC;
+  g.near = 1;
+  for (const RecView &v : g.in) g.near &= v.st * (long long)sizeof(T) == (int)(v.st * (long long)sizeof(T));
+  for (const RecView &v : g.out) g.near &= v.st * (long long)sizeof(T) == (int)(v.st * (long long)sizeof(T));
   const long long blocks = (g.groups + 31) / 32;
   // as many warps a block and blocks a cluster as there are spans for, until
   // two blocks an SM are there
-  const long long spans = (g.steps + N - 1) / N;
+  const long long spans = ((long long)g.steps + N - 1) / N;
   int warps = 1, ranks = 1;
   while (warps < mmpd::kRecWarps && warps < spans) warps *= 2;
   while (ranks < 8 && blocks * ranks < 2 * mmp::sm_count() && (long long)ranks * warps < spans) ranks *= 2;
@@ -432,7 +483,7 @@ int mmp_recurrence(int dtype, int gated, int64_t outer, int64_t steps, int64_t i
   g.out[0] = RecView{h, h_so, h_st};
   g.h0 = g.seed = h0;
   g.last = state;
-  g.steps = steps;
+  g.steps = (int)steps;
   return gated ? rec_dispatch<false, true>(dtype, g, chains, inner) : rec_dispatch<false, false>(dtype, g, chains, inner);
 }
 
@@ -458,7 +509,7 @@ int mmp_recurrence_grad(int dtype, int gated, int64_t outer, int64_t steps, int6
   r.h0 = h0;
   r.seed = grad_state;
   r.last = grad_h0;
-  r.steps = steps;
+  r.steps = (int)steps;
   return gated ? rec_dispatch<true, true>(dtype, r, chains, inner) : rec_dispatch<true, false>(dtype, r, chains, inner);
 }
 
