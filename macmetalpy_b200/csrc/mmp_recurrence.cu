@@ -96,6 +96,42 @@ __device__ __forceinline__ void rec_wait(int n) {
   else asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
+// The cluster's exchange: st.async writes into the other blocks' shared memory
+// and counts its bytes on a barrier there.  A fence in its place (the release
+// of barrier.cluster) waits for this block's own loads and stores on the way,
+// the ring's loads ahead among them: 314 us against 302 for 1 x 65521 x 1000
+// float32.
+__device__ __forceinline__ unsigned rec_map(const void *p, int rank) {
+  unsigned r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"((unsigned)__cvta_generic_to_shared(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void rec_send(unsigned dst, unsigned bar, float a, float h) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(dst),
+               "f"(a), "f"(h), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void rec_send(unsigned dst, unsigned bar, double a, double h) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.f64 [%0], {%1, %2}, [%3];" ::"r"(dst),
+               "d"(a), "d"(h), "r"(bar)
+               : "memory");
+}
+// Waits for the barrier's phase; false if it has not come after a second or so.
+__device__ __forceinline__ bool rec_arrived(unsigned bar, unsigned phase) {
+  for (unsigned n = 0; n < (1u << 23); ++n) {
+    unsigned ok;
+    asm volatile(
+        "{\n.reg .pred p;\nmbarrier.test_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n"
+        "selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(phase)
+        : "memory");
+    if (ok) return true;
+    if (n > 256) __nanosleep(64);
+  }
+  return false;
+}
+
 struct RecArgs {
   RecView in[4];   // forward: a, x; backward: a, grad, h, x
   RecView out[2];  // forward: h; backward: grad_a, grad_x
@@ -105,6 +141,7 @@ struct RecArgs {
   long long groups, per;  // per: groups along inner
   int steps, iters, stages;
   int near;  // every step stride is below 2^31 bytes
+  int *err;
 };
 
 constexpr int kRecWarps = 8;
@@ -118,7 +155,12 @@ template <class S> struct alignas(2 * sizeof(S)) RecMap {
   S a, h;
 };
 
-template <class T, int VEC, bool GRAD, bool GATED, bool CLUSTER>
+// How a span's rows reach the ring.  kWide: the warp copies them in 16-byte
+// pieces, several rows an instruction, past L1 (the others take 4 or 8 bytes a
+// lane, whose lines on the way are held in what the ring leaves of L1).
+enum { kPlain, kLane, kWide };
+
+template <class T, int VEC, int COPY, bool GRAD, bool GATED, bool CLUSTER>
 __global__ void __launch_bounds__(32 * kRecWarps, 2) rec_kernel(const __grid_constant__ RecArgs g) {
   typedef typename RecState<T>::type S;
   typedef RecVec<T, VEC> V;
@@ -126,11 +168,14 @@ __global__ void __launch_bounds__(32 * kRecWarps, 2) rec_kernel(const __grid_con
   constexpr int NA = GRAD ? (GATED ? 4 : 3) : 2;
   constexpr int NO = GRAD ? 2 : 1;
   constexpr int NC = 32 * VEC;            // chains of the block
-  constexpr bool ASYNC = sizeof(V) >= 4;  // cp.async copies 4, 8 or 16 bytes
+  constexpr bool ASYNC = COPY != kPlain;
+  constexpr int PIECE = 16 / (int)sizeof(T);             // elements
+  constexpr int PER = NC / PIECE, ROWS = 32 / PER;        // pieces a row, rows an instruction
   extern __shared__ __align__(16) unsigned char s_ring[];
   __shared__ RecMap<S> s_map[kRecWarps][NC];                         // the warps' spans
   __shared__ RecMap<S> s_blk[CLUSTER ? 2 : 1][CLUSTER ? 8 : 1][NC];  // the cluster's blocks' spans
   __shared__ S s_start[kRecWarps][NC], s_carry[NC];
+  __shared__ __align__(8) unsigned long long s_bar[2];
   const int lane = threadIdx.x, w = threadIdx.y, warps = blockDim.y;
   int rank = 0, ranks = 1;
   long long blk = blockIdx.x;
@@ -138,16 +183,29 @@ __global__ void __launch_bounds__(32 * kRecWarps, 2) rec_kernel(const __grid_con
     rank = (int)cg::this_cluster().block_rank();
     ranks = (int)cg::this_cluster().num_blocks();
     blk = blockIdx.x / ranks;
-    // every block of the cluster has to run before its shared memory is written
-    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    // every block of the cluster has to run, its barriers set up, before it is sent anything
+    if (w == 0 && lane < 2)
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"((unsigned)__cvta_generic_to_shared(&s_bar[lane]))
+                   : "memory");
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   }
   const long long grp = blk * 32 + lane;
   const bool active = grp < g.groups;
   const long long o = active ? grp / g.per : 0;
   const long long i = active ? (grp - o * g.per) * VEC : 0;
+  // where this lane copies from: its own chains, or its piece of the warp's
+  const long long cg0 = COPY == kWide ? blk * 32 * VEC + lane % PER * PIECE : 0;  // first chain of the piece
+  const bool copies = COPY == kWide ? cg0 < g.groups * VEC : active;
   const T *in[NA];
+  if (COPY == kWide) {
+    const long long co = copies ? cg0 / (g.per * VEC) : 0, ci = copies ? cg0 - co * (g.per * VEC) : 0;
 #pragma unroll
-  for (int q = 0; q < NA; ++q) in[q] = (const T *)g.in[q].p + o * g.in[q].so + i;
+    for (int q = 0; q < NA; ++q) in[q] = (const T *)g.in[q].p + co * g.in[q].so + ci;
+  } else {
+#pragma unroll
+    for (int q = 0; q < NA; ++q) in[q] = (const T *)g.in[q].p + o * g.in[q].so + i;
+  }
   T *out[NO];
 #pragma unroll
   for (int q = 0; q < NO; ++q) out[q] = (T *)const_cast<void *>(g.out[q].p) + o * g.out[q].so + i;
@@ -167,10 +225,26 @@ __global__ void __launch_bounds__(32 * kRecWarps, 2) rec_kernel(const __grid_con
   V pre[ASYNC ? 1 : NA][ASYNC ? 1 : N];
   auto issue = [&](int it) {
     const int k0 = it * span + mine;
-    const int left = active ? g.steps - k0 : 0;
+    const int left = copies ? g.steps - k0 : 0;
     if (left <= 0) return;
     const unsigned slot = (unsigned)__cvta_generic_to_shared(ring + (ASYNC ? it % g.stages : 0) * (NA * N * 32));
     const long long t0 = GRAD ? g.steps - 1 - k0 : k0;
+    if constexpr (COPY == kWide) {
+      const int row = lane / PER;
+      const unsigned dst = slot - lane * (int)sizeof(V) + row * (NC * (int)sizeof(T)) + lane % PER * 16;
+#pragma unroll
+      for (int q = 0; q < NA; ++q) {
+        const long long st = (GRAD ? -g.in[q].st : g.in[q].st) * ROWS;
+        const T *p = in[q] + ((GRAD && q == 2 ? t0 - 1 : t0) + (GRAD ? -row : row)) * g.in[q].st;
+        const int n = (GRAD && q == 2 ? left - 1 : left) - row;
+#pragma unroll
+        for (int j = 0; j < N; j += ROWS) {
+          if (j < n) rec_cp_async<16>(dst + (q * N + j) * (NC * (int)sizeof(T)), p);
+          p += st;
+        }
+      }
+      return;
+    }
     if (left > N && g.near) {  // a whole span with one address instruction a step
 #pragma unroll
       for (int q = 0; q < NA; ++q) {
@@ -209,13 +283,16 @@ __global__ void __launch_bounds__(32 * kRecWarps, 2) rec_kernel(const __grid_con
   } else {
     issue(0);
   }
-  if (CLUSTER) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+  if (CLUSTER) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  bool heard = true;
 
   for (int it = 0; it < g.iters; ++it) {
     if constexpr (ASYNC) {
+      if (COPY == kWide) __syncwarp();  // every lane is done with the stage that is filled next
       if (it + ahead < g.iters) issue(it + ahead);
       rec_commit();
       rec_wait(ahead);
+      if (COPY == kWide) __syncwarp();  // the other lanes' pieces too
     } else {
 #pragma unroll
       for (int q = 0; q < NA; ++q)
@@ -268,6 +345,11 @@ __global__ void __launch_bounds__(32 * kRecWarps, 2) rec_kernel(const __grid_con
       __syncthreads();
       const int tid = w * 32 + lane, par = it & 1;
       if (CLUSTER) {
+        const unsigned bar = (unsigned)__cvta_generic_to_shared(&s_bar[par]);
+        if (tid == 0)
+          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar),
+                       "r"(ranks * NC * (int)sizeof(RecMap<S>))
+                       : "memory");
         for (int c = tid; c < NC; c += 32 * warps) {
           RecMap<S> m = s_map[0][c];
           for (int b = 1; b < warps; ++b) {
@@ -275,10 +357,12 @@ __global__ void __launch_bounds__(32 * kRecWarps, 2) rec_kernel(const __grid_con
             m.h = rec_apply(n.a, n.h, m.h);
             m.a *= n.a;
           }
-          for (int r = 0; r < ranks; ++r) *cg::this_cluster().map_shared_rank(&s_blk[par][rank][c], r) = m;
+          for (int r = 0; r < ranks; ++r) rec_send(rec_map(&s_blk[par][rank][c], r), rec_map(&s_bar[par], r), m.a, m.h);
         }
-        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (tid < NC && heard) {
+          heard = rec_arrived(bar, (it >> 1) & 1);
+          if (!heard) atomicExch(g.err, 9);
+        }
       }
       for (int c = tid; c < NC; c += 32 * warps) {
         S st = s_carry[c];
@@ -370,6 +454,10 @@ __global__ void __launch_bounds__(32 * kRecWarps, 2) rec_kernel(const __grid_con
       }
     }
   }
+  if (CLUSTER) {  // no block ends while it may still be sent to
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+  }
   if (g.steps == 0 && g.last && active && w == 0) {
 #pragma unroll
     for (int v = 0; v < VEC; ++v) ((S *)g.last)[grp * VEC + v] = carry[v];
@@ -394,9 +482,9 @@ int rec_sizes(const char *what, int dtype, int64_t outer, int64_t steps, int64_t
   return MMP_OK;
 }
 
-template <class T, int VEC, bool GRAD, bool GATED, bool CLUSTER>
+template <class T, int VEC, int COPY, bool GRAD, bool GATED, bool CLUSTER>
 int rec_launch(const RecArgs &g, unsigned blocks, int warps, int ranks, size_t smem) {
-  auto fn = mmpd::rec_kernel<T, VEC, GRAD, GATED, CLUSTER>;
+  auto fn = mmpd::rec_kernel<T, VEC, COPY, GRAD, GATED, CLUSTER>;
   if (smem > 32 * 1024)  // together with the static part this can pass the default 48 KB
     MMP_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   cudaLaunchConfig_t cfg = {};
@@ -416,29 +504,31 @@ int rec_launch(const RecArgs &g, unsigned blocks, int warps, int ranks, size_t s
   return MMP_OK;
 }
 
-template <class T, int VEC, bool GRAD, bool GATED>
+template <class T, int VEC, int COPY, bool GRAD, bool GATED>
 int rec_run(RecArgs g, long long chains, long long inner) {
   constexpr int N = mmpd::RecSpan<(int)sizeof(T) * VEC, GRAD>::value;
   constexpr int NA = GRAD ? (GATED ? 4 : 3) : 2;
   g.groups = chains / VEC;
   g.per = inner / VEC;
+  g.err = mmp::device_error_word();
   g.near = 1;
   for (const RecView &v : g.in) g.near &= v.st * (long long)sizeof(T) == (int)(v.st * (long long)sizeof(T));
   for (const RecView &v : g.out) g.near &= v.st * (long long)sizeof(T) == (int)(v.st * (long long)sizeof(T));
   const long long blocks = (g.groups + 31) / 32;
-  // as many warps a block and blocks a cluster as there are spans for, until
-  // two blocks an SM are there
+  // as many warps a block and blocks a cluster as there are spans for, while
+  // all blocks fit at two an SM: 8 x 2048 x 2048 float16 (256 blocks) takes 46
+  // us in blocks alone and 59 in clusters of two, which run in two waves;
+  // 1 x 65521 x 1000 float32 (32 blocks) 606 alone and 186 in clusters of eight
   const long long spans = ((long long)g.steps + N - 1) / N;
   int warps = 1, ranks = 1;
   while (warps < mmpd::kRecWarps && warps < spans) warps *= 2;
-  while (ranks < 8 && blocks * ranks < 2 * mmp::sm_count() && (long long)ranks * warps < spans) ranks *= 2;
+  while (ranks < 8 && blocks * ranks * 2 <= 2 * mmp::sm_count() && (long long)ranks * warps < spans) ranks *= 2;
   if (blocks * ranks > INT32_MAX) return mmp::set_error(MMP_E_ARG, "recurrence: too many chains");
   g.iters = (int)((spans + (long long)warps * ranks - 1) / ((long long)warps * ranks));
-  constexpr bool async = sizeof(T) * VEC >= 4;
-  g.stages = async ? (g.iters < 3 ? (g.iters > 0 ? g.iters : 1) : 3) : 1;
+  g.stages = COPY != mmpd::kPlain ? (g.iters < 3 ? (g.iters > 0 ? g.iters : 1) : 3) : 1;
   const size_t smem = (size_t)g.stages * NA * N * warps * 32 * sizeof(T) * VEC;
-  return ranks > 1 ? rec_launch<T, VEC, GRAD, GATED, true>(g, (unsigned)blocks, warps, ranks, smem)
-                   : rec_launch<T, VEC, GRAD, GATED, false>(g, (unsigned)blocks, warps, ranks, smem);
+  return ranks > 1 ? rec_launch<T, VEC, COPY, GRAD, GATED, true>(g, (unsigned)blocks, warps, ranks, smem)
+                   : rec_launch<T, VEC, COPY, GRAD, GATED, false>(g, (unsigned)blocks, warps, ranks, smem);
 }
 
 // Whether every operand can be moved in pieces of `bytes` (e: element size).
@@ -456,12 +546,18 @@ bool rec_aligned(const RecArgs &g, int nin, int nout, long long inner, size_t by
 template <bool GRAD, bool GATED>
 int rec_dispatch(int dtype, const RecArgs &g, long long chains, long long inner) {
   constexpr int nin = GRAD ? (GATED ? 4 : 3) : 2, nout = GRAD ? 2 : 1;
+  using namespace mmpd;
+  const size_t e = mmp_dtype_size(dtype);
+  const bool wide = rec_aligned(g, nin, nout, inner, 16, e);
   if (dtype == MMP_FLOAT16) {
-    if (rec_aligned(g, nin, nout, inner, 4, 2)) return rec_run<__half, 2, GRAD, GATED>(g, chains, inner);
-    return rec_run<__half, 1, GRAD, GATED>(g, chains, inner);
+    if (wide) return rec_run<__half, 2, kWide, GRAD, GATED>(g, chains, inner);
+    if (rec_aligned(g, nin, nout, inner, 4, e)) return rec_run<__half, 2, kLane, GRAD, GATED>(g, chains, inner);
+    return rec_run<__half, 1, kPlain, GRAD, GATED>(g, chains, inner);
   }
-  if (dtype == MMP_FLOAT32) return rec_run<float, 1, GRAD, GATED>(g, chains, inner);
-  return rec_run<double, 1, GRAD, GATED>(g, chains, inner);
+  if (dtype == MMP_FLOAT32)
+    return wide ? rec_run<float, 1, kWide, GRAD, GATED>(g, chains, inner)
+                : rec_run<float, 1, kLane, GRAD, GATED>(g, chains, inner);
+  return rec_run<double, 1, kLane, GRAD, GATED>(g, chains, inner);
 }
 
 }  // namespace

@@ -51,7 +51,7 @@ def gates(a, gated):
 
 def grow(a, gated):
     """K, per element."""
-    return 16 + (2.4 * np.minimum(np.abs(a.astype(np.float64)), 104) if gated and a.dtype == np.float16 else 0 * a)
+    return 16 + (2.4 * np.minimum(np.abs(a.astype(np.float64)), 104) if gated and a.dtype == np.float16 else np.zeros(a.shape))
 
 
 def recurrence(a, x, h0, gated):
