@@ -19,17 +19,26 @@
 //   block    `warps` spans after one another, joined through shared memory
 //   cluster  its blocks' spans after one another, joined through each
 //            other's shared memory; then the cluster moves on along the axis
+// A span's steps run twice, once to compose it and once, from the state then
+// known, for the outputs.  One more warp of the block joins the spans; where
+// the gates need not stay in registers in between, the others compose the
+// next span before they replay the last and do not wait for it.
 // Every input is read once and every output written once; no block waits for
 // one outside its cluster, nothing is allocated, and the order of all
 // operations is fixed by the sizes.  What bounds it is HBM traffic, so the
 // loads run ahead: each thread copies the steps of its next spans with
 // cp.async into a ring in shared memory that only it reads.
 #include <cooperative_groups.h>
+#include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include "mmp_device.cuh"
 #include "mmp_internal.h"
+
+namespace mmp {
+void *driver_fn(const char *name);
+}
 
 namespace mmpd {
 
@@ -82,6 +91,17 @@ template <class S> __device__ __forceinline__ S rec_apply(S A, S H, S s) { retur
 
 template <class T, int VEC> struct alignas(sizeof(T) * VEC) RecVec { T v[VEC]; };
 
+// A store that the compiler knows to be global (its pointer comes out of a
+// structure), so that it does not hold back the loads from the ring after it.
+template <class V> __device__ __forceinline__ void rec_store(void *p, const V &v) {
+  if constexpr (sizeof(V) == 2)
+    asm volatile("st.global.b16 [%0], %1;" ::"l"(p), "h"(*reinterpret_cast<const unsigned short *>(&v)));
+  else if constexpr (sizeof(V) == 4)
+    asm volatile("st.global.b32 [%0], %1;" ::"l"(p), "r"(*reinterpret_cast<const unsigned *>(&v)));
+  else
+    asm volatile("st.global.b64 [%0], %1;" ::"l"(p), "l"(*reinterpret_cast<const unsigned long long *>(&v)));
+}
+
 template <int BYTES> __device__ __forceinline__ void rec_cp_async(unsigned dst, const void *src) {
   if (BYTES == 16)
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -91,9 +111,14 @@ template <int BYTES> __device__ __forceinline__ void rec_cp_async(unsigned dst, 
 __device__ __forceinline__ void rec_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // Waits until at most `n` of this thread's newest groups are still on the way.
 __device__ __forceinline__ void rec_wait(int n) {
-  if (n >= 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
-  else if (n == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
-  else asm volatile("cp.async.wait_group 0;" ::: "memory");
+  switch (n) {
+    case 0: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
+    case 1: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
+    case 2: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
+    case 3: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
+    case 4: asm volatile("cp.async.wait_group 4;" ::: "memory"); break;
+    default: asm volatile("cp.async.wait_group 5;" ::: "memory"); break;
+  }
 }
 
 // The cluster's exchange: st.async writes into the other blocks' shared memory
@@ -132,19 +157,28 @@ __device__ __forceinline__ bool rec_arrived(unsigned bar, unsigned phase) {
   return false;
 }
 
+// Named barriers of the block: 1 and 2, a span's compositions are there; 3
+// and 4, the states before them are.
+__device__ __forceinline__ void rec_bar_sync(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+__device__ __forceinline__ void rec_bar_arrive(int id, int threads) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
 struct RecArgs {
   RecView in[4];   // forward: a, x; backward: a, grad, h, x
   RecView out[2];  // forward: h; backward: grad_a, grad_x
   const void *h0;
   const void *seed;  // the state before the first span: h0 / grad_state
   void *last;        // the state after the last span: state / grad_h0
-  long long groups, per;  // per: groups along inner
-  int steps, iters, stages;
+  long long outer, inner, tiles;  // tiles: of 32 VEC chains along inner
+  int steps, iters, stages, warps;
   int near;  // every step stride is below 2^31 bytes
   int *err;
 };
 
-constexpr int kRecWarps = 8;
+constexpr int kRecWarps = 7;  // and one that joins them: 8 warps of 128 registers, two blocks an SM
 
 // Steps of one warp's span, by the bytes that a lane moves a step: 32 KB of
 // ring a stage and block of 8 warps, so that two blocks of three stages fit an
@@ -155,28 +189,49 @@ template <class S> struct alignas(2 * sizeof(S)) RecMap {
   S a, h;
 };
 
-// How a span's rows reach the ring.  kWide: the warp copies them in 16-byte
-// pieces, several rows an instruction, past L1 (the others take 4 or 8 bytes a
-// lane, whose lines on the way are held in what the ring leaves of L1).
-enum { kPlain, kLane, kWide };
+// How a span's rows reach the ring.  kTma: one tensor copy an array, by one
+// lane of the warp.  kLane: cp.async of each lane's own 4 or 8 bytes (any
+// strides; issuing these takes a third of the warps' time, and their lines on
+// the way are held in what the ring leaves of L1).  kPlain: loads of 2 bytes,
+// for float16 in rows of odd width.
+enum { kPlain, kLane, kTma };
+
+template <int COPY> struct RecMaps {};
+struct alignas(64) RecMap3 {
+  CUtensorMap m;
+  int swap;  // (inner, outer, steps) in place of (inner, steps, outer)
+};
+template <> struct RecMaps<kTma> {
+  RecMap3 in[4];
+};
+
+__device__ __forceinline__ void rec_tma(unsigned dst, const RecMap3 &map, unsigned bar, int i, int t, int o) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+          dst),
+      "l"(&map.m), "r"(bar), "r"(i), "r"(map.swap ? o : t), "r"(map.swap ? t : o)
+      : "memory");
+}
 
 template <class T, int VEC, int COPY, bool GRAD, bool GATED, bool CLUSTER>
-__global__ void __launch_bounds__(32 * kRecWarps, 2) rec_kernel(const __grid_constant__ RecArgs g) {
+__global__ void __launch_bounds__(32 * (kRecWarps + 1), 2) rec_kernel(
+    const __grid_constant__ RecArgs g, const __grid_constant__ RecMaps<COPY> maps) {
   typedef typename RecState<T>::type S;
   typedef RecVec<T, VEC> V;
   constexpr int N = RecSpan<(int)sizeof(V), GRAD>::value;
   constexpr int NA = GRAD ? (GATED ? 4 : 3) : 2;
   constexpr int NO = GRAD ? 2 : 1;
   constexpr int NC = 32 * VEC;            // chains of the block
-  constexpr bool ASYNC = COPY != kPlain;
-  constexpr int PIECE = 16 / (int)sizeof(T);             // elements
-  constexpr int PER = NC / PIECE, ROWS = 32 / PER;        // pieces a row, rows an instruction
-  extern __shared__ __align__(16) unsigned char s_ring[];
-  __shared__ RecMap<S> s_map[kRecWarps][NC];                         // the warps' spans
-  __shared__ RecMap<S> s_blk[CLUSTER ? 2 : 1][CLUSTER ? 8 : 1][NC];  // the cluster's blocks' spans
-  __shared__ S s_start[kRecWarps][NC], s_carry[NC];
-  __shared__ __align__(8) unsigned long long s_bar[2];
-  const int lane = threadIdx.x, w = threadIdx.y, warps = blockDim.y;
+  constexpr bool ASYNC = COPY == kLane;
+  constexpr int kStages = 3;
+  extern __shared__ __align__(128) unsigned char s_ring[];
+  constexpr bool HOLD = GATED && !CLUSTER;  // gates of a span stay in registers from compose to replay
+  constexpr int LAG = HOLD ? 0 : 1;         // spans between compose and replay
+  __shared__ __align__(16) RecMap<S> s_map[2][kRecWarps][NC];                      // the warps' spans
+  __shared__ __align__(16) RecMap<S> s_blk[CLUSTER ? 2 : 1][CLUSTER ? 8 : 1][NC];  // the cluster's blocks' spans
+  __shared__ __align__(16) S s_start[2][kRecWarps][NC];                            // states before the warps' spans
+  __shared__ __align__(8) unsigned long long s_bar[2], s_full[kRecWarps][kStages];
+  const int lane = threadIdx.x, w = threadIdx.y, warps = g.warps;
   int rank = 0, ranks = 1;
   long long blk = blockIdx.x;
   if (CLUSTER) {
@@ -190,61 +245,138 @@ __global__ void __launch_bounds__(32 * kRecWarps, 2) rec_kernel(const __grid_con
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   }
-  const long long grp = blk * 32 + lane;
-  const bool active = grp < g.groups;
-  const long long o = active ? grp / g.per : 0;
-  const long long i = active ? (grp - o * g.per) * VEC : 0;
-  // where this lane copies from: its own chains, or its piece of the warp's
-  const long long cg0 = COPY == kWide ? blk * 32 * VEC + lane % PER * PIECE : 0;  // first chain of the piece
-  const bool copies = COPY == kWide ? cg0 < g.groups * VEC : active;
-  const T *in[NA];
-  if (COPY == kWide) {
-    const long long co = copies ? cg0 / (g.per * VEC) : 0, ci = copies ? cg0 - co * (g.per * VEC) : 0;
-#pragma unroll
-    for (int q = 0; q < NA; ++q) in[q] = (const T *)g.in[q].p + co * g.in[q].so + ci;
+  // the lane's chains: of a row of tiles for tensor copies, else of all groups in a row
+  long long o, i;
+  bool active;
+  if constexpr (COPY == kTma) {
+    o = blk / g.tiles;
+    i = (blk - o * g.tiles) * NC + lane * VEC;
+    active = i < g.inner;
   } else {
-#pragma unroll
-    for (int q = 0; q < NA; ++q) in[q] = (const T *)g.in[q].p + o * g.in[q].so + i;
+    const long long grp = blk * 32 + lane, per = g.inner / VEC;
+    active = grp < g.outer * per;
+    o = active ? grp / per : 0;
+    i = active ? (grp - o * per) * VEC : 0;
   }
+  const long long chain = o * g.inner + i;
+  const T *in[NA];
+#pragma unroll
+  for (int q = 0; q < NA; ++q) in[q] = (const T *)g.in[q].p + o * g.in[q].so + i;
   T *out[NO];
 #pragma unroll
   for (int q = 0; q < NO; ++q) out[q] = (T *)const_cast<void *>(g.out[q].p) + o * g.out[q].so + i;
   // this thread's slots: [stage][array][step], a row of 32 lanes each
-  V *const ring = reinterpret_cast<V *>(s_ring) + (size_t)w * g.stages * (NA * N * 32) + lane;
+  // (tensor copies go to multiples of 128 bytes)
+  const unsigned skew = (unsigned)(-(int)__cvta_generic_to_shared(s_ring)) & 127u;
+  V *const ring = reinterpret_cast<V *>(s_ring + skew) + (size_t)w * g.stages * (NA * N * 32) + lane;
   const int span = ranks * warps * N;  // steps of the cluster
   const int mine = (rank * warps + w) * N;
-  S carry[VEC];  // the state before the present span of a block of one warp
+  S carry[VEC];  // the state before the present span of the cluster (joining warp; a block of one warp)
 #pragma unroll
-  for (int v = 0; v < VEC; ++v) {
-    carry[v] = active && g.seed ? ((const S *)g.seed)[grp * VEC + v] : S(0);
-    if (w == 0) s_carry[lane * VEC + v] = carry[v];
+  for (int v = 0; v < VEC; ++v) carry[v] = active && g.seed ? ((const S *)g.seed)[chain + v] : S(0);
+
+  if (w == warps) {
+    // The joining warp, beside the warps that compose and replay: a lane has
+    // the chains of its group.
+    if (CLUSTER) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    bool heard = true;
+    for (int it = 0; it < g.iters; ++it) {
+      const int par = it & 1;
+      rec_bar_sync(1 + par, 32 * (warps + 1));
+      RecMap<S> m[kRecWarps][VEC];
+#pragma unroll
+      for (int b = 0; b < kRecWarps; ++b)
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) m[b][v] = b < warps ? s_map[par][b][lane * VEC + v] : RecMap<S>{S(1), S(0)};
+      S st[VEC];
+      if (CLUSTER) {
+        // This block's composition to every block of the cluster, and theirs
+        // back.  Two places are enough: a block sends for it + 2 once it has
+        // everyone's of it + 1, which each sent after reading it's.
+        RecMap<S> all[VEC];
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+          all[v] = m[0][v];
+#pragma unroll
+          for (int b = 1; b < kRecWarps; ++b) {
+            all[v].h = rec_apply(m[b][v].a, m[b][v].h, all[v].h);
+            all[v].a *= m[b][v].a;
+          }
+        }
+        const unsigned bar = (unsigned)__cvta_generic_to_shared(&s_bar[par]);
+        if (lane == 0)
+          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar),
+                       "r"(ranks * NC * (int)sizeof(RecMap<S>))
+                       : "memory");
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          if (r < ranks) {
+            const unsigned to = rec_map(&s_blk[par][rank][lane * VEC], r), tob = rec_map(&s_bar[par], r);
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) rec_send(to + v * (int)sizeof(RecMap<S>), tob, all[v].a, all[v].h);
+          }
+        }
+        if (heard) {
+          heard = rec_arrived(bar, (it >> 1) & 1);
+          if (!heard) atomicExch(g.err, 9);
+        }
+        RecMap<S> n[8][VEC];
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+#pragma unroll
+          for (int v = 0; v < VEC; ++v)
+            n[r][v] = r < ranks ? s_blk[par][CLUSTER ? r : 0][lane * VEC + v] : RecMap<S>{S(1), S(0)};
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+#pragma unroll
+          for (int r = 0; r < 8; ++r) {
+            if (r == rank) st[v] = carry[v];
+            carry[v] = rec_apply(n[r][v].a, n[r][v].h, carry[v]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) st[v] = carry[v];
+      }
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {
+#pragma unroll
+        for (int b = 0; b < kRecWarps; ++b) {
+          if (b < warps) s_start[par][b][lane * VEC + v] = st[v];
+          st[v] = rec_apply(m[b][v].a, m[b][v].h, st[v]);
+        }
+        if (!CLUSTER) carry[v] = st[v];
+      }
+      rec_bar_arrive(3 + par, 32 * (warps + 1));
+    }
+    if (CLUSTER) {
+      asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+      asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    }
+    return;
   }
 
   // step k in the order of work lies at t = k forward, steps - 1 - k backward;
   // h is read one step before, so at t = 0 (where h0 stands in) not at all
   V pre[ASYNC ? 1 : NA][ASYNC ? 1 : N];
-  auto issue = [&](int it) {
+  auto issue = [&](int it, int stage) {
     const int k0 = it * span + mine;
-    const int left = copies ? g.steps - k0 : 0;
+    const int left = active || COPY == kTma ? g.steps - k0 : 0;
     if (left <= 0) return;
-    const unsigned slot = (unsigned)__cvta_generic_to_shared(ring + (ASYNC ? it % g.stages : 0) * (NA * N * 32));
-    const long long t0 = GRAD ? g.steps - 1 - k0 : k0;
-    if constexpr (COPY == kWide) {
-      const int row = lane / PER;
-      const unsigned dst = slot - lane * (int)sizeof(V) + row * (NC * (int)sizeof(T)) + lane % PER * 16;
+    const unsigned slot = (unsigned)__cvta_generic_to_shared(ring + stage * (NA * N * 32));
+    if constexpr (COPY == kTma) {  // called by lane 0; rows in order of time, steps outside the axis read as zeros
+      const unsigned full = (unsigned)__cvta_generic_to_shared(&s_full[w][stage]);
+      const int t0 = GRAD ? g.steps - k0 - N : k0;
+      asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full),
+                   "r"(NA * N * 32 * (int)sizeof(V))
+                   : "memory");
 #pragma unroll
-      for (int q = 0; q < NA; ++q) {
-        const long long st = (GRAD ? -g.in[q].st : g.in[q].st) * ROWS;
-        const T *p = in[q] + ((GRAD && q == 2 ? t0 - 1 : t0) + (GRAD ? -row : row)) * g.in[q].st;
-        const int n = (GRAD && q == 2 ? left - 1 : left) - row;
-#pragma unroll
-        for (int j = 0; j < N; j += ROWS) {
-          if (j < n) rec_cp_async<16>(dst + (q * N + j) * (NC * (int)sizeof(T)), p);
-          p += st;
-        }
-      }
+      for (int q = 0; q < NA; ++q)
+        rec_tma(slot + q * N * 32 * (int)sizeof(V), maps.in[q], full, (int)(i / NC) * NC, GRAD && q == 2 ? t0 - 1 : t0,
+                (int)o);
       return;
     }
+    const long long t0 = GRAD ? g.steps - 1 - k0 : k0;
     if (left > N && g.near) {  // a whole span with one address instruction a step
 #pragma unroll
       for (int q = 0; q < NA; ++q) {
@@ -274,55 +406,54 @@ __global__ void __launch_bounds__(32 * kRecWarps, 2) rec_kernel(const __grid_con
       }
     }
   };
-  const int ahead = ASYNC ? g.stages - 1 : 0;
-  if constexpr (ASYNC) {
+  // stages that are filled ahead: all but the one in work and, with a lag,
+  // the one that is replayed (unless every span has its own)
+  const int ahead = COPY == kPlain ? 0 : g.stages - (LAG && warps > 1 && g.stages < g.iters ? 2 : 1);
+  bool heard = true;
+  if constexpr (COPY == kTma) {
+    if (lane == 0) {
+      for (int q = 0; q < kStages; ++q)
+        asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"((unsigned)__cvta_generic_to_shared(&s_full[w][q]))
+                     : "memory");
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+      for (int it = 0; it < ahead; ++it) issue(it, it);
+    }
+    __syncwarp();
+  } else if constexpr (ASYNC) {
     for (int it = 0; it < ahead; ++it) {
-      issue(it);
+      issue(it, it);
       rec_commit();
     }
   } else {
-    issue(0);
+    issue(0, 0);
   }
   if (CLUSTER) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-  bool heard = true;
 
-  for (int it = 0; it < g.iters; ++it) {
-    if constexpr (ASYNC) {
-      if (COPY == kWide) __syncwarp();  // every lane is done with the stage that is filled next
-      if (it + ahead < g.iters) issue(it + ahead);
-      rec_commit();
-      rec_wait(ahead);
-      if (COPY == kWide) __syncwarp();  // the other lanes' pieces too
-    } else {
-#pragma unroll
-      for (int q = 0; q < NA; ++q)
-#pragma unroll
-        for (int j = 0; j < N; ++j) ring[(q * N + j) * 32] = pre[q][j];
-      if (it + 1 < g.iters) issue(it + 1);
-    }
-    const int k0 = it * span + mine;
-    const int left = active ? g.steps - k0 : 0;
-    const V *const slot = ring + (ASYNC ? it % g.stages : 0) * (NA * N * 32);
+  auto row = [](int j) { return COPY == kTma && GRAD ? N - 1 - j : j; };  // where the ring has a step
+  constexpr int M = N < 8 ? N : 8;  // steps whose ring entries are read at once
+  S F[HOLD ? N : 1][VEC], U[HOLD ? N : 1][VEC];  // f and u forward, f and 1 - f backward
+  S A[VEC], H[VEC], s[VEC];
 
-    // the span's composition, from a state of zero.  Gates are evaluated once
-    // and kept: f and u forward, f and 1 - f backward.
-    S F[GATED ? N : 1][VEC], U[GATED ? N : 1][VEC], A[VEC], H[VEC];
+  // the composition of a span's steps: the state after them, from zero
+  auto compose = [&](int it, int stage) {
+    const int left = active ? g.steps - (it * span + mine) : 0;
+    const V *const slot = ring + stage * (NA * N * 32);
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
       A[v] = S(1);
       H[v] = S(0);
     }
-    auto compose = [&](int j) {
-      const V va = slot[j * 32], vb = slot[(N + j) * 32];
+    auto step = [&](int j, const V &va, const V &vb) {
 #pragma unroll
       for (int v = 0; v < VEC; ++v) {
-        S f = Cvt<S, T>::f(va.v[v]), u = Cvt<S, T>::f(vb.v[v]);
-        if constexpr (GATED) {
-          S rest;
+        S f = Cvt<S, T>::f(va.v[v]), u = Cvt<S, T>::f(vb.v[v]), rest;
+        if (GATED) {
           rec_gate<T>(f, f, rest);
+          if (!GRAD) u *= rest;
+        }
+        if constexpr (HOLD) {
           F[j][v] = f;
-          U[j][v] = GRAD ? rest : rest * u;
-          if (!GRAD) u = U[j][v];
+          U[j][v] = GRAD ? rest : u;
         }
         H[v] = GRAD ? f * (u + H[v]) : fma(f, H[v], u);
         A[v] *= f;
@@ -330,106 +461,79 @@ __global__ void __launch_bounds__(32 * kRecWarps, 2) rec_kernel(const __grid_con
     };
     if (left >= N) {
 #pragma unroll
-      for (int j = 0; j < N; ++j) compose(j);
+      for (int j0 = 0; j0 < N; j0 += M) {
+        V va[M], vb[M];
+#pragma unroll
+        for (int j = 0; j < M; ++j) {
+          va[j] = slot[row(j0 + j) * 32];
+          vb[j] = slot[(N + row(j0 + j)) * 32];
+        }
+#pragma unroll
+        for (int j = 0; j < M; ++j) step(j0 + j, va[j], vb[j]);
+      }
     } else {
 #pragma unroll
       for (int j = 0; j < N; ++j)
-        if (j < left) compose(j);
+        if (j < left) step(j, slot[row(j) * 32], slot[(N + row(j)) * 32]);
     }
+  };
 
-    // join the block's warps, then the cluster's blocks: one thread a chain
-    S s[VEC];
-    if (warps > 1 || CLUSTER) {
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) s_map[w][lane * VEC + v] = RecMap<S>{A[v], H[v]};
-      __syncthreads();
-      const int tid = w * 32 + lane, par = it & 1;
-      if (CLUSTER) {
-        const unsigned bar = (unsigned)__cvta_generic_to_shared(&s_bar[par]);
-        if (tid == 0)
-          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar),
-                       "r"(ranks * NC * (int)sizeof(RecMap<S>))
-                       : "memory");
-        for (int c = tid; c < NC; c += 32 * warps) {
-          RecMap<S> m = s_map[0][c];
-          for (int b = 1; b < warps; ++b) {
-            const RecMap<S> n = s_map[b][c];
-            m.h = rec_apply(n.a, n.h, m.h);
-            m.a *= n.a;
-          }
-          for (int r = 0; r < ranks; ++r) rec_send(rec_map(&s_blk[par][rank][c], r), rec_map(&s_bar[par], r), m.a, m.h);
-        }
-        if (tid < NC && heard) {
-          heard = rec_arrived(bar, (it >> 1) & 1);
-          if (!heard) atomicExch(g.err, 9);
-        }
-      }
-      for (int c = tid; c < NC; c += 32 * warps) {
-        S st = s_carry[c];
-        if (CLUSTER) {
-          S at = st;
-          for (int r = 0; r < ranks; ++r) {
-            if (r == rank) at = st;
-            st = rec_apply(s_blk[par][r][c].a, s_blk[par][r][c].h, st);
-          }
-          s_carry[c] = st;
-          st = at;
-        }
-        for (int b = 0; b < warps; ++b) {
-          s_start[b][c] = st;
-          st = rec_apply(s_map[b][c].a, s_map[b][c].h, st);
-        }
-        if (!CLUSTER) s_carry[c] = st;
-      }
-      __syncthreads();
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) s[v] = s_start[w][lane * VEC + v];
-    } else {
+  // its steps again, from the state s before them, with the outputs
+  auto replay = [&](int it, int stage) {
+    const int k0 = it * span + mine;
+    const int left = active ? g.steps - k0 : 0;
+    const V *const slot = ring + stage * (NA * N * 32);
+    struct Row {
+      V a, b, h, x;
+    };
+    auto read = [&](int j, bool first) {
+      Row w;
+      if (!HOLD) w.a = slot[row(j) * 32];
+      if (GRAD || !HOLD) w.b = slot[(N + row(j)) * 32];
+      if (GRAD && !first) w.h = slot[(2 * N + row(j)) * 32];
+      if (GRAD && GATED) w.x = slot[((NA - 1) * N + row(j)) * 32];
+      return w;
+    };
+    auto step = [&](int j, const Row &w, bool first, V &r0, V &r1) {
+      const V &va = w.a, &vb = w.b, &vh = w.h, &vx = w.x;
 #pragma unroll
       for (int v = 0; v < VEC; ++v) {
-        s[v] = carry[v];
-        carry[v] = rec_apply(A[v], H[v], carry[v]);
-      }
-    }
-
-    // the span's steps again, from the state before it
-    auto replay = [&](int j, bool first, V &r0, V &r1) {
-      V va, vb, vh, vx;
-      if (GRAD || !GATED) vb = slot[(N + j) * 32];
-      if (!GATED) va = slot[j * 32];
-      if (GRAD && !first) vh = slot[(2 * N + j) * 32];
-      if (GRAD && GATED) vx = slot[((NA - 1) * N + j) * 32];
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        const S f = GATED ? F[GATED ? j : 0][v] : Cvt<S, T>::f(va.v[v]);
+        S f, rest, u;
+        if constexpr (HOLD) {
+          f = F[j][v];
+          rest = u = U[j][v];
+        } else {
+          f = Cvt<S, T>::f(va.v[v]);
+          if (GATED) rec_gate<T>(f, f, rest);
+          if (!GRAD) u = GATED ? rest * Cvt<S, T>::f(vb.v[v]) : Cvt<S, T>::f(vb.v[v]);
+        }
         if (!GRAD) {
-          s[v] = fma(f, s[v], GATED ? U[GATED ? j : 0][v] : Cvt<S, T>::f(vb.v[v]));
+          s[v] = fma(f, s[v], u);
           r0.v[v] = Cvt<T, S>::f(s[v]);
         } else {
           const S gt = Cvt<S, T>::f(vb.v[v]) + s[v];
-          const S hp = !first ? Cvt<S, T>::f(vh.v[v]) : g.h0 ? ((const S *)g.h0)[grp * VEC + v] : S(0);
-          if constexpr (GATED) {
-            const S rest = U[j][v];
-            r0.v[v] = Cvt<T, S>::f(gt * (hp - Cvt<S, T>::f(vx.v[v])) * (f * rest));
-            r1.v[v] = Cvt<T, S>::f(gt * rest);
-          } else {
-            r0.v[v] = Cvt<T, S>::f(gt * hp);
-            r1.v[v] = Cvt<T, S>::f(gt);
-          }
+          const S hp = !first ? Cvt<S, T>::f(vh.v[v]) : g.h0 ? ((const S *)g.h0)[chain + v] : S(0);
+          r0.v[v] = Cvt<T, S>::f(GATED ? gt * (hp - Cvt<S, T>::f(vx.v[v])) * (f * rest) : gt * hp);
+          r1.v[v] = Cvt<T, S>::f(GATED ? gt * rest : gt);
           s[v] = f * gt;
         }
       }
     };
     const long long t0 = GRAD ? g.steps - 1 - k0 : k0;
+    Row rows[M];
     if (left > N && g.near) {  // whole, and not the last span
 #pragma unroll
       for (int j = 0; j < N; ++j) {
+        if (j % M == 0) {
+#pragma unroll
+          for (int i = 0; i < M; ++i) rows[i] = read(j + i, false);
+        }
         V r[2];
-        replay(j, false, r[0], r[1]);
+        step(j, rows[j % M], false, r[0], r[1]);
 #pragma unroll
         for (int q = 0; q < NO; ++q) {
           const int st = (int)(GRAD ? -g.out[q].st : g.out[q].st) * (int)sizeof(T);
-          *reinterpret_cast<V *>((char *)(out[q] + t0 * g.out[q].st) + (long long)st * j) = r[q];
+          rec_store((char *)(out[q] + t0 * g.out[q].st) + (long long)st * j, r[q]);
         }
       }
     } else if (left > 0) {
@@ -440,17 +544,74 @@ __global__ void __launch_bounds__(32 * kRecWarps, 2) rec_kernel(const __grid_con
       for (int j = 0; j < N; ++j) {
         if (j < left) {
           V r[2];
-          replay(j, GRAD && j + 1 == left, r[0], r[1]);
+          const bool first = GRAD && j + 1 == left;
+          step(j, read(j, first), first, r[0], r[1]);
 #pragma unroll
           for (int q = 0; q < NO; ++q) {
-            *reinterpret_cast<V *>(po[q]) = r[q];
+            rec_store(po[q], r[q]);
             po[q] += GRAD ? -g.out[q].st : g.out[q].st;
           }
         }
       }
       if (left <= N && g.last) {
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) ((S *)g.last)[grp * VEC + v] = s[v];
+        for (int v = 0; v < VEC; ++v) ((S *)g.last)[chain + v] = s[v];
+      }
+    }
+  };
+
+  // stages in turn: of the span filled next, composed next, replayed next
+  int fill = ahead % g.stages, next = 0, last = 0;
+  unsigned phase = 0;
+  for (int it = 0; it < g.iters + (warps > 1 ? LAG : 0); ++it) {
+    if (it < g.iters) {
+      if constexpr (COPY == kTma) {
+        __syncwarp();  // every lane is done with the stage that is filled next
+        if (lane == 0 && it + ahead < g.iters) issue(it + ahead, fill);
+        if (heard && it * span + mine < g.steps) {
+          heard = rec_arrived((unsigned)__cvta_generic_to_shared(&s_full[w][next]), phase);
+          if (!heard) atomicExch(g.err, 9);
+        }
+      } else if constexpr (ASYNC) {
+        if (it + ahead < g.iters) issue(it + ahead, fill);
+        rec_commit();
+        rec_wait(ahead);
+      } else {
+        V *const slot = ring + next * (NA * N * 32);
+#pragma unroll
+        for (int q = 0; q < NA; ++q)
+#pragma unroll
+          for (int j = 0; j < N; ++j) slot[(q * N + j) * 32] = pre[q][j];
+        if (it + 1 < g.iters) issue(it + 1, 0);
+      }
+      compose(it, next);
+      if (++fill == g.stages) fill = 0;
+      if (++next == g.stages) {
+        next = 0;
+        phase ^= 1;
+      }
+    }
+    if (warps == 1) {
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {
+        s[v] = carry[v];
+        carry[v] = rec_apply(A[v], H[v], carry[v]);
+      }
+      replay(it, last);
+      if (++last == g.stages) last = 0;
+    } else {
+      if (it < g.iters) {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) s_map[it & 1][w][lane * VEC + v] = RecMap<S>{A[v], H[v]};
+        rec_bar_arrive(1 + (it & 1), 32 * (warps + 1));
+      }
+      if (it >= LAG) {
+        const int par = (it - LAG) & 1;
+        rec_bar_sync(3 + par, 32 * (warps + 1));
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) s[v] = s_start[par][w][lane * VEC + v];
+        replay(it - LAG, last);
+        if (++last == g.stages) last = 0;
       }
     }
   }
@@ -460,7 +621,7 @@ __global__ void __launch_bounds__(32 * kRecWarps, 2) rec_kernel(const __grid_con
   }
   if (g.steps == 0 && g.last && active && w == 0) {
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) ((S *)g.last)[grp * VEC + v] = carry[v];
+    for (int v = 0; v < VEC; ++v) ((S *)g.last)[chain + v] = carry[v];
   }
 }
 
@@ -483,13 +644,13 @@ int rec_sizes(const char *what, int dtype, int64_t outer, int64_t steps, int64_t
 }
 
 template <class T, int VEC, int COPY, bool GRAD, bool GATED, bool CLUSTER>
-int rec_launch(const RecArgs &g, unsigned blocks, int warps, int ranks, size_t smem) {
+int rec_launch(const RecArgs &g, const mmpd::RecMaps<COPY> &maps, unsigned blocks, int ranks, size_t smem) {
   auto fn = mmpd::rec_kernel<T, VEC, COPY, GRAD, GATED, CLUSTER>;
-  if (smem > 32 * 1024)  // together with the static part this can pass the default 48 KB
+  if (smem > 16 * 1024)  // together with the static part this can pass the default 48 KB
     MMP_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(blocks * ranks);
-  cfg.blockDim = dim3(32, warps);
+  cfg.blockDim = dim3(32, g.warps + (g.warps > 1));  // and the joining warp
   cfg.dynamicSmemBytes = smem;
   cfg.stream = mmp::stream();
   cudaLaunchAttribute at[1];
@@ -500,41 +661,95 @@ int rec_launch(const RecArgs &g, unsigned blocks, int warps, int ranks, size_t s
     cfg.attrs = at;
     cfg.numAttrs = 1;
   }
-  MMP_CUDA_TRY(cudaLaunchKernelEx(&cfg, fn, g));
+  MMP_CUDA_TRY(cudaLaunchKernelEx(&cfg, fn, g, maps));
+  return MMP_OK;
+}
+
+// Byte strides of the second and third axis of a tensor map, as its
+// documentation wants them: multiples of 16 below 2^40, the first at least a
+// row, the second a multiple of the first.  An axis of one entry takes one
+// that fits.
+struct RecStrides {
+  long long s1, s2;
+  bool swap;
+};
+bool rec_strides(const RecView &v, const RecArgs &g, long long e, RecStrides *s) {
+  const long long most = 1ll << 40, row = g.inner * e;
+  if (v.st >= most / e || v.so >= most / e) return false;
+  long long st = v.st * e, so = v.so * e;
+  if (g.outer == 1) so = (g.steps == 1 ? (row + 15) / 16 * 16 : st) * g.steps;
+  if (g.steps == 1) st = g.outer == 1 ? (row + 15) / 16 * 16 : so;
+  s->swap = so < st;
+  s->s1 = s->swap ? so : st;
+  s->s2 = s->swap ? st : so;
+  return s->s1 >= row && s->s1 > 0 && s->s1 % 16 == 0 && s->s2 % s->s1 == 0 && s->s2 < most;
+}
+
+typedef CUresult (*PFN_Encode)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                               const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                               CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// A map over (inner, steps, outer), or (inner, outer, steps) where the steps
+// lie further apart, with boxes of chains x steps.
+int rec_map_of(mmpd::RecMap3 *map, const RecView &v, const RecArgs &g, int e, int chains, int steps) {
+  static const PFN_Encode enc = (PFN_Encode)mmp::driver_fn("cuTensorMapEncodeTiled");
+  if (!enc) return mmp::set_error(MMP_E_CUDA, "cuTensorMapEncodeTiled unavailable");
+  RecStrides s;
+  if (!rec_strides(v, g, e, &s)) return mmp::set_error(MMP_E_ARG, "recurrence: strides of a tensor copy");
+  const bool swap = map->swap = s.swap;
+  const cuuint64_t dims[3] = {(cuuint64_t)g.inner, (cuuint64_t)(swap ? g.outer : g.steps),
+                              (cuuint64_t)(swap ? g.steps : g.outer)};
+  const cuuint64_t strides[2] = {(cuuint64_t)s.s1, (cuuint64_t)s.s2};
+  const cuuint32_t box[3] = {(cuuint32_t)chains, (cuuint32_t)(swap ? 1 : steps), (cuuint32_t)(swap ? steps : 1)};
+  const cuuint32_t one[3] = {1, 1, 1};
+  const CUresult r = enc(&map->m, e == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3,
+                         const_cast<void *>(v.p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return mmp::set_error(MMP_E_CUDA, "recurrence: cuTensorMapEncodeTiled failed");
   return MMP_OK;
 }
 
 template <class T, int VEC, int COPY, bool GRAD, bool GATED>
-int rec_run(RecArgs g, long long chains, long long inner) {
+int rec_run(RecArgs g) {
   constexpr int N = mmpd::RecSpan<(int)sizeof(T) * VEC, GRAD>::value;
   constexpr int NA = GRAD ? (GATED ? 4 : 3) : 2;
-  g.groups = chains / VEC;
-  g.per = inner / VEC;
+  constexpr int NC = 32 * VEC;
   g.err = mmp::device_error_word();
   g.near = 1;
   for (const RecView &v : g.in) g.near &= v.st * (long long)sizeof(T) == (int)(v.st * (long long)sizeof(T));
   for (const RecView &v : g.out) g.near &= v.st * (long long)sizeof(T) == (int)(v.st * (long long)sizeof(T));
-  const long long blocks = (g.groups + 31) / 32;
+  g.tiles = (g.inner + NC - 1) / NC;
+  const long long blocks = COPY == mmpd::kTma ? g.outer * g.tiles : (g.outer * (g.inner / VEC) + 31) / 32;
   // as many warps a block and blocks a cluster as there are spans for, while
   // all blocks fit at two an SM: 8 x 2048 x 2048 float16 (256 blocks) takes 46
   // us in blocks alone and 59 in clusters of two, which run in two waves;
   // 1 x 65521 x 1000 float32 (32 blocks) 606 alone and 186 in clusters of eight
   const long long spans = ((long long)g.steps + N - 1) / N;
   int warps = 1, ranks = 1;
-  while (warps < mmpd::kRecWarps && warps < spans) warps *= 2;
+  if (spans > 1) warps = spans < mmpd::kRecWarps ? (int)spans : mmpd::kRecWarps;
   while (ranks < 8 && blocks * ranks * 2 <= 2 * mmp::sm_count() && (long long)ranks * warps < spans) ranks *= 2;
   if (blocks * ranks > INT32_MAX) return mmp::set_error(MMP_E_ARG, "recurrence: too many chains");
   g.iters = (int)((spans + (long long)warps * ranks - 1) / ((long long)warps * ranks));
-  g.stages = COPY != mmpd::kPlain ? (g.iters < 3 ? (g.iters > 0 ? g.iters : 1) : 3) : 1;
-  const size_t smem = (size_t)g.stages * NA * N * warps * 32 * sizeof(T) * VEC;
-  return ranks > 1 ? rec_launch<T, VEC, COPY, GRAD, GATED, true>(g, (unsigned)blocks, warps, ranks, smem)
-                   : rec_launch<T, VEC, COPY, GRAD, GATED, false>(g, (unsigned)blocks, warps, ranks, smem);
+  g.warps = warps;
+  const int most = COPY != mmpd::kPlain ? 3 : warps > 1 ? 2 : 1;
+  g.stages = g.iters < most ? (g.iters > 0 ? g.iters : 1) : most;
+  const size_t smem = 128 + (size_t)g.stages * NA * N * warps * 32 * sizeof(T) * VEC;
+  mmpd::RecMaps<COPY> maps;
+  if constexpr (COPY == mmpd::kTma) {
+    for (int q = 0; q < NA; ++q) {
+      const int rc = rec_map_of(&maps.in[q], g.in[q], g, (int)sizeof(T), NC, N);
+      if (rc) return rc;
+    }
+  }
+  return ranks > 1 ? rec_launch<T, VEC, COPY, GRAD, GATED, true>(g, maps, (unsigned)blocks, ranks, smem)
+                   : rec_launch<T, VEC, COPY, GRAD, GATED, false>(g, maps, (unsigned)blocks, ranks, smem);
 }
 
 // Whether every operand can be moved in pieces of `bytes` (e: element size).
-bool rec_aligned(const RecArgs &g, int nin, int nout, long long inner, size_t bytes, size_t e) {
+bool rec_aligned(const RecArgs &g, int nin, int nout, size_t bytes, size_t e) {
   const long long vec = (long long)(bytes / e);
-  if (inner % vec) return false;
+  if (g.inner % vec) return false;
   auto ok = [&](const RecView &v) { return (uintptr_t)v.p % bytes == 0 && v.so % vec == 0 && v.st % vec == 0; };
   for (int i = 0; i < nin; ++i)
     if (!ok(g.in[i])) return false;
@@ -543,21 +758,30 @@ bool rec_aligned(const RecArgs &g, int nin, int nout, long long inner, size_t by
   return true;
 }
 
+// Whether tensor copies can take the inputs, and their tiles of `chains` along
+// inner are at least three quarters full.
+bool rec_tensors(const RecArgs &g, int nin, int chains, long long e) {
+  if (g.steps == 0 || g.inner * 4 < (g.inner + chains - 1) / chains * chains * 3) return false;
+  if (g.inner > INT32_MAX || g.outer > INT32_MAX) return false;
+  RecStrides s;
+  for (int i = 0; i < nin; ++i)
+    if ((uintptr_t)g.in[i].p % 16 || !rec_strides(g.in[i], g, e, &s)) return false;
+  return true;
+}
+
 template <bool GRAD, bool GATED>
-int rec_dispatch(int dtype, const RecArgs &g, long long chains, long long inner) {
-  constexpr int nin = GRAD ? (GATED ? 4 : 3) : 2, nout = GRAD ? 2 : 1;
+int rec_dispatch(int dtype, const RecArgs &g) {
   using namespace mmpd;
-  const size_t e = mmp_dtype_size(dtype);
-  const bool wide = rec_aligned(g, nin, nout, inner, 16, e);
+  constexpr int nin = GRAD ? (GATED ? 4 : 3) : 2, nout = GRAD ? 2 : 1;
   if (dtype == MMP_FLOAT16) {
-    if (wide) return rec_run<__half, 2, kWide, GRAD, GATED>(g, chains, inner);
-    if (rec_aligned(g, nin, nout, inner, 4, e)) return rec_run<__half, 2, kLane, GRAD, GATED>(g, chains, inner);
-    return rec_run<__half, 1, kPlain, GRAD, GATED>(g, chains, inner);
+    if (!rec_aligned(g, nin, nout, 4, 2)) return rec_run<__half, 1, kPlain, GRAD, GATED>(g);
+    return rec_tensors(g, nin, 64, 2) ? rec_run<__half, 2, kTma, GRAD, GATED>(g)
+                                      : rec_run<__half, 2, kLane, GRAD, GATED>(g);
   }
   if (dtype == MMP_FLOAT32)
-    return wide ? rec_run<float, 1, kWide, GRAD, GATED>(g, chains, inner)
-                : rec_run<float, 1, kLane, GRAD, GATED>(g, chains, inner);
-  return rec_run<double, 1, kLane, GRAD, GATED>(g, chains, inner);
+    return rec_tensors(g, nin, 32, 4) ? rec_run<float, 1, kTma, GRAD, GATED>(g)
+                                      : rec_run<float, 1, kLane, GRAD, GATED>(g);
+  return rec_run<double, 1, kLane, GRAD, GATED>(g);
 }
 
 }  // namespace
@@ -580,7 +804,9 @@ int mmp_recurrence(int dtype, int gated, int64_t outer, int64_t steps, int64_t i
   g.h0 = g.seed = h0;
   g.last = state;
   g.steps = (int)steps;
-  return gated ? rec_dispatch<false, true>(dtype, g, chains, inner) : rec_dispatch<false, false>(dtype, g, chains, inner);
+  g.outer = outer;
+  g.inner = inner;
+  return gated ? rec_dispatch<false, true>(dtype, g) : rec_dispatch<false, false>(dtype, g);
 }
 
 int mmp_recurrence_grad(int dtype, int gated, int64_t outer, int64_t steps, int64_t inner, const void *a, int64_t a_so,
@@ -606,7 +832,9 @@ int mmp_recurrence_grad(int dtype, int gated, int64_t outer, int64_t steps, int6
   r.seed = grad_state;
   r.last = grad_h0;
   r.steps = (int)steps;
-  return gated ? rec_dispatch<true, true>(dtype, r, chains, inner) : rec_dispatch<true, false>(dtype, r, chains, inner);
+  r.outer = outer;
+  r.inner = inner;
+  return gated ? rec_dispatch<true, true>(dtype, r) : rec_dispatch<true, false>(dtype, r);
 }
 
 }  // extern "C"

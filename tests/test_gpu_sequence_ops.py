@@ -237,6 +237,29 @@ def test_recurrence_axes_and_views(cp, dt, axis):
                                   cp.linear_recurrence(one.copy(), cp.array(x), axis=axis).get())
 
 
+@pytest.mark.parametrize("dt", ["float16", "float32"])
+def test_recurrence_time_major_and_skipped_steps(cp, dt):
+    """Memory in (steps, batch, width) order, every second step of an odd
+    number, every second batch entry, one step and one batch entry."""
+    rng = np.random.default_rng(6)
+    base = rng.standard_normal((61, 4, 192)).astype(dt)
+    B = cp.array(base)
+    views = [lambda v: v[..., :96].transpose(1, 0, 2), lambda v: v[..., :96][::2].transpose(1, 0, 2),
+             lambda v: v[:, ::2, :64].transpose(1, 0, 2), lambda v: v[:1, :, :64].transpose(1, 0, 2),
+             lambda v: v[:, 1:2, :64].transpose(1, 0, 2), lambda v: v[::-1, :, :64].transpose(1, 0, 2),
+             lambda v: v[1::2], lambda v: v[3:4]]
+    for f in views:
+        a, x = f(base), f(base[..., 96:] if f(base).shape[2] < 192 else base)
+        hs, es, _, _ = recurrence(a, x, None, True)
+        va, vx = f(B), f(B[..., 96:] if f(base).shape[2] < 192 else B)
+        h = cp.linear_recurrence(va, vx, gated=True)
+        close(h.get(), hs, es * UNIT[dt], dt)
+        da, dx, _, ea, ex, _ = recurrence_grad(a, x, h.get(), x, None, None, True)
+        got = cp.linear_recurrence_grad(va, vx, h, vx, gated=True)
+        close(got[0].get(), da, ea * UNIT[dt], dt)
+        close(got[1].get(), dx, ex * UNIT[dt], dt)
+
+
 @pytest.mark.parametrize("off", range(1, 8))
 @pytest.mark.parametrize("dt", ["float16", "float32"])
 def test_recurrence_unaligned_views(cp, dt, off):
