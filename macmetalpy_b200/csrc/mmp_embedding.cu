@@ -1,13 +1,24 @@
 // mmp_embedding / mmp_embedding_grad: rows of a table by token id, times a
 // scale, and the gradient of the table,
 //   out[n, :] = scale * weight[ids[n], :]
-//   grad_weight[v, :] = scale * sum over n with ids[n] = v, in order of n, of grad[n, :].
+//   grad_weight[v, :] = scale * sum over n with ids[n] = v of grad[n, :].
 // The reference has take (indexing.py:24-60; numpy on the host) without a
 // scale or a gradient.  Products and sums are in float32 (float64 for
-// float64 tables) and each output is rounded once.
+// float64 tables) and each output is rounded once.  An id outside [0, rows)
+// gives a row of zeros in the lookup, adds nothing in the gradient, and sets
+// device error 5, as mmp_gather does for an offset.
 //
-// An id outside [0, rows) gives a row of zeros in the lookup, adds nothing in
-// the gradient, and sets device error 5, as mmp_gather does for an offset.
+// Both are bound by HBM traffic.  The gradient reads each row of grad once
+// and writes each row of the table once, zeros included, whatever the ids:
+//   few tokens   one launch: a block a token, which adds its id's rows if it
+//                is the first with that id; other blocks write the zeros of
+//                the rows without a token.
+//   more         the tokens are sorted by id (stable, so the order of every
+//                sum is the ids' alone) by one cluster while the rest of the
+//                GPU writes the zeros; then equal shares of the sorted tokens
+//                are added run by run, and runs that cross shares are joined.
+// No float is added atomically, so equal calls give equal bits.
+#include <cooperative_groups.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -16,49 +27,483 @@
 
 namespace mmpd {
 
+namespace cg = cooperative_groups;
+
 template <class T> struct EmbAcc { typedef float type; };
 template <> struct EmbAcc<double> { typedef double type; };
 
-template <class T, class I>
-__global__ void __launch_bounds__(256) emb_kernel(const T *__restrict__ w, long long rows, long long width,
-                                                  long long w_stride, const I *__restrict__ ids, long long n,
+template <class T, int VEC> struct alignas(sizeof(T) * VEC) EmbVec { T v[VEC]; };
+
+// ---- lookup: a thread moves U vectors; vectors of a row are neighbours.
+template <class T, class I, int VEC, int U>
+__global__ void __launch_bounds__(256) emb_kernel(const T *__restrict__ w, long long rows, FastDiv per,
+                                                  long long w_stride, const I *__restrict__ ids, unsigned total,
                                                   typename EmbAcc<T>::type scale, T *__restrict__ out, int *err) {
   typedef typename EmbAcc<T>::type S;
-  for (long long r = blockIdx.x; r < n; r += gridDim.x) {
-    const long long id = (long long)ids[r];
-    const bool ok = id >= 0 && id < rows;
-    if (!ok && threadIdx.x == 0) atomicExch(err, 5);
-    for (long long j = threadIdx.x; j < width; j += blockDim.x)
-      out[r * width + j] = ok ? Cvt<T, S>::f((S)Cvt<S, T>::f(w[id * w_stride + j]) * scale) : Cvt<T, S>::f(S(0));
+  typedef EmbVec<T, VEC> V;
+  const unsigned i0 = blockIdx.x * (256u * U) + threadIdx.x;
+  unsigned col[U];
+  long long id[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const unsigned i = i0 + u * 256u;
+    const unsigned r = per.div(i);
+    col[u] = i - r * per.d;
+    id[u] = i < total ? (long long)ids[r] : -1;
+  }
+  V v[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const unsigned i = i0 + u * 256u;
+    const bool ok = id[u] >= 0 && id[u] < rows;
+    if (i < total && !ok) atomicExch(err, 5);
+    if (ok) {
+      v[u] = *reinterpret_cast<const V *>(w + id[u] * w_stride + (long long)col[u] * VEC);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[u].v[e] = Cvt<T, S>::f(S(0));
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const unsigned i = i0 + u * 256u;
+    if (i >= total) break;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[u].v[e] = Cvt<T, S>::f(Cvt<S, T>::f(v[u].v[e]) * scale);
+    *reinterpret_cast<V *>(out + (long long)i * VEC) = v[u];
   }
 }
 
-// One warp per row of the table walks the ids and adds the rows of the
-// gradient that are its own, 32 columns at a time.
+// ---- zeros of the rows [r0, r1) that no token has, by one block.  s_seen: a
+// bitmap of at least r1 - r0 bits.  The rows are one stretch of memory,
+// written in 16-byte pieces; a piece that belongs to two rows, or sticks out
+// at an end, goes element by element.
 template <class T, class I>
-__global__ void __launch_bounds__(256) emb_grad_kernel(const I *__restrict__ ids, long long n, const T *__restrict__ grad,
-                                                       long long g_stride, long long rows, long long width,
-                                                       typename EmbAcc<T>::type scale, long long padding,
-                                                       T *__restrict__ out, int *err) {
+__device__ void emb_zero_rows(const I *__restrict__ ids, unsigned n, long long rows, long long padding, long long r0,
+                              long long r1, FastDiv width, T *__restrict__ out, unsigned *s_seen, int *err) {
+  const unsigned tid = threadIdx.x, nt = blockDim.x;
+  const unsigned count = (unsigned)(r1 - r0);
+  __syncthreads();
+  for (unsigned i = tid; i < (count + 31) / 32; i += nt) s_seen[i] = 0;
+  __syncthreads();
+#pragma unroll 4
+  for (unsigned i = tid; i < n; i += nt) {
+    const long long id = (long long)ids[i];
+    if (id >= r0 && id < r1 && id != padding) atomicOr(&s_seen[(id - r0) >> 5], 1u << ((id - r0) & 31));
+    if (r0 == 0 && (id < 0 || id >= rows)) atomicExch(err, 5);
+  }
+  __syncthreads();
+  auto seen = [&](unsigned r) { return (s_seen[r >> 5] >> (r & 31)) & 1u; };
+  // in parts of rows whose elements 32 bits count
+  const unsigned part = 0x7fffffffu / width.d > count ? count : 0x7fffffffu / width.d ? 0x7fffffffu / width.d : 1;
+  constexpr unsigned PE = 16 / sizeof(T);
+  const T zero = Cvt<T, float>::f(0.0f);
+  for (unsigned p0 = 0; p0 < count; p0 += part) {
+    T *base = out + (r0 + p0) * width.d;
+    const unsigned elems = (count - p0 < part ? count - p0 : part) * width.d;
+    const unsigned head = (unsigned)((16 - ((uintptr_t)base & 15)) & 15) / (unsigned)sizeof(T);
+    const unsigned pieces = elems > head ? (elems - head) / PE : 0;
+    const unsigned tail = elems > head ? head + pieces * PE : 0;  // elements outside: [0, head) and [tail, elems)
+    for (unsigned i = tid; i < pieces; i += nt) {
+      const unsigned e = head + i * PE;
+      const unsigned ra = width.div(e), rb = width.div(e + PE - 1);
+      bool a = seen(p0 + ra), b = seen(p0 + rb);
+      if (rb > ra + 1) a = true;  // rows shorter than a piece
+      if (!a && !b) {
+        *reinterpret_cast<uint4 *>(base + e) = make_uint4(0, 0, 0, 0);
+      } else if (ra != rb) {
+        for (unsigned j = 0; j < PE; ++j)
+          if (!seen(p0 + width.div(e + j))) base[e + j] = zero;
+      }
+    }
+    const unsigned h = head < elems ? head : elems;
+    for (unsigned e = tid; e < h; e += nt)
+      if (!seen(p0 + width.div(e))) base[e] = zero;
+    if (elems > head)
+      for (unsigned e = tail + tid; e < elems; e += nt)
+        if (!seen(p0 + width.div(e))) base[e] = zero;
+  }
+}
+
+// This block's part of the rows, in stretches of at most `bits` rows.
+template <class T, class I>
+__device__ __forceinline__ void emb_zero_share(const I *ids, unsigned n, long long rows, long long padding, unsigned part,
+                                               unsigned parts, unsigned bits, FastDiv width, T *out, unsigned *s_seen,
+                                               int *err) {
+  const long long share = (rows + parts - 1) / parts;
+  const long long a = share * part, b = a + share < rows ? a + share : rows;
+  for (long long r = a; r < b; r += bits)
+    emb_zero_rows<T, I>(ids, n, rows, padding, r, r + bits < b ? r + bits : b, width, out, s_seen, err);
+}
+
+constexpr unsigned kEmbFew = 1024;       // tokens up to which no sort is made
+constexpr unsigned kEmbFewBits = 16384;  // rows a block of that path marks at once
+
+// ---- few tokens, one launch.  Blocks [0, n): token blockIdx.x, if it is the
+// first of its id, adds all of them in the order of n.  The others: zeros.
+template <class T, class I, int VEC>
+__global__ void __launch_bounds__(256) emb_grad_few(const I *__restrict__ ids, unsigned n, const T *__restrict__ grad,
+                                                    long long g_stride, long long rows, FastDiv width,
+                                                    typename EmbAcc<T>::type scale, long long padding,
+                                                    T *__restrict__ out, int *err) {
   typedef typename EmbAcc<T>::type S;
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
-  if (blockIdx.x == 0)
-    for (long long i = threadIdx.x; i < n; i += blockDim.x) {
+  typedef EmbVec<T, VEC> V;
+  __shared__ unsigned s_buf[kEmbFew];  // the list of tokens, or the bitmap
+  __shared__ unsigned s_sum[8];
+  const unsigned tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  if (blockIdx.x >= n) {
+    emb_zero_share<T, I>(ids, n, rows, padding, blockIdx.x - n, gridDim.x - n, kEmbFewBits, width, out, s_buf, err);
+    return;
+  }
+  const unsigned me = blockIdx.x;
+  const long long id = (long long)ids[me];
+  if (id < 0 || id >= rows) {
+    if (tid == 0) atomicExch(err, 5);
+    return;
+  }
+  if (id == padding) return;
+  // the tokens of this id in order, 4 places a thread
+  unsigned hit = 0, count = 0;
+  bool earlier = false;
+#pragma unroll
+  for (unsigned u = 0; u < kEmbFew / 256; ++u) {
+    const unsigned i = tid * (kEmbFew / 256) + u;
+    if (i < n && (long long)ids[i] == id) {
+      hit |= 1u << u;
+      ++count;
+      earlier |= i < me;
+    }
+  }
+  if (__syncthreads_or(earlier)) return;
+  unsigned before = count;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned t = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += t;
+  }
+  if (lane == 31) s_sum[w] = before;
+  __syncthreads();
+  unsigned total = 0;
+  before -= count;
+#pragma unroll
+  for (unsigned v = 0; v < 8; ++v) {
+    if (v < w) before += s_sum[v];
+    total += s_sum[v];
+  }
+#pragma unroll
+  for (unsigned u = 0; u < kEmbFew / 256; ++u)
+    if (hit >> u & 1) s_buf[before++] = tid * (kEmbFew / 256) + u;
+  __syncthreads();
+  for (unsigned c = tid * VEC; c < width.d; c += 256 * VEC) {
+    S acc[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) acc[e] = S(0);
+    unsigned k = 0;
+    for (; k + 8 <= total; k += 8) {
+      V v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = *reinterpret_cast<const V *>(grad + s_buf[k + j] * g_stride + c);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) acc[e] += Cvt<S, T>::f(v[j].v[e]);
+    }
+    for (; k < total; ++k) {
+      const V v = *reinterpret_cast<const V *>(grad + s_buf[k] * g_stride + c);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) acc[e] += Cvt<S, T>::f(v.v[e]);
+    }
+    V r;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) r.v[e] = Cvt<T, S>::f(acc[e] * scale);
+    *reinterpret_cast<V *>(out + id * width.d + c) = r;
+  }
+}
+
+// ---- the sort of up to kEmbCluster tokens by one cluster, beside the zeros.
+constexpr int kSortThreads = 1024, kSortRanks = 8, kSortItems = 8;
+constexpr unsigned kEmbCluster = kSortThreads * kSortRanks * kSortItems;  // 65536
+struct EmbSortSmem {
+  unsigned count[32][256];          // a warp's keys of each digit
+  unsigned total[kSortRanks][256];  // each block's
+  unsigned base[256];
+  unsigned sum[8];
+  unsigned long long key[2][1];  // E * 1024 each: id << 32 | token
+};
+
+__device__ __forceinline__ unsigned emb_lanemask_lt() {
+  unsigned m;
+  asm("mov.u32 %0, %%lanemask_lt;" : "=r"(m));
+  return m;
+}
+
+// Cluster 0 sorts (LSD radix: a block has E * 1024 neighbouring keys in its
+// shared memory, a warp E * 32 of them; keys go to their place in the next
+// pass through the cluster's shared memory).  A key that counts for no row
+// (padding, out of range) is `rows`.  The other clusters write zeros.
+template <class T, class I>
+__global__ void __cluster_dims__(kSortRanks, 1, 1) __launch_bounds__(kSortThreads, 1)
+    emb_sort_kernel(const I *__restrict__ ids, unsigned n, long long rows, long long padding, int items, int passes,
+                    int digit, unsigned *__restrict__ keys, unsigned *__restrict__ order, FastDiv width,
+                    T *__restrict__ out, unsigned bits, int *err) {
+  extern __shared__ __align__(16) unsigned char s_raw[];
+  if (blockIdx.x >= kSortRanks) {
+    emb_zero_share<T, I>(ids, n, rows, padding, blockIdx.x - kSortRanks, gridDim.x - kSortRanks, bits, width, out,
+                         (unsigned *)s_raw, err);
+    return;
+  }
+  EmbSortSmem &s = *reinterpret_cast<EmbSortSmem *>(s_raw);
+  cg::cluster_group cl = cg::this_cluster();
+  const unsigned rank = cl.block_rank();
+  const unsigned tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  const unsigned tile = items * kSortThreads;
+  unsigned long long *const buf[2] = {s.key[0], s.key[0] + tile};
+  const unsigned place = w * items * 32 + lane;  // this thread's keys: place + 32 e
+  const unsigned lt = emb_lanemask_lt();
+  for (int e = 0; e < items; ++e) {
+    const unsigned p = place + e * 32, i = rank * tile + p;
+    if (i < n) {
       const long long id = (long long)ids[i];
-      if (id < 0 || id >= rows) atomicExch(err, 5);
+      const bool ok = id >= 0 && id < rows;
+      if (!ok) atomicExch(err, 5);
+      buf[0][p] = (unsigned long long)(ok && id != padding ? id : rows) << 32 | i;
     }
-  for (long long v = (long long)blockIdx.x * nw + w; v < rows; v += (long long)gridDim.x * nw) {
-    for (long long j0 = 0; j0 < width; j0 += 32) {
-      const long long j = j0 + lane;
-      S acc = S(0);
-      if (v != padding)
-        for (long long i0 = 0; i0 < n; i0 += 32) {
-          unsigned m = __ballot_sync(0xffffffffu, i0 + lane < n && (long long)ids[i0 + lane] == v);
-          for (; m; m &= m - 1)
-            if (j < width) acc += Cvt<S, T>::f(grad[(i0 + __ffs(m) - 1) * g_stride + j]);
+  }
+  for (int pass = 0; pass < passes; ++pass) {
+    const int shift = 32 + pass * digit;
+    const unsigned mask = (1u << digit) - 1;
+    unsigned long long *from = buf[pass & 1];
+    for (unsigned j = tid; j < 32 * 256; j += kSortThreads) (&s.count[0][0])[j] = 0;
+    __syncthreads();
+    unsigned long long k[kSortItems];
+    unsigned at[kSortItems];
+#pragma unroll
+    for (int e = 0; e < kSortItems; ++e) {
+      if (e < items) {
+        const bool valid = rank * tile + place + e * 32 < n;
+        k[e] = valid ? from[place + e * 32] : 0;
+        const unsigned d = (unsigned)(k[e] >> shift) & mask;
+        unsigned peers = __ballot_sync(0xffffffffu, valid);
+        for (int b = 0; b < digit; ++b) {
+          const bool bit = (d >> b) & 1u;
+          const unsigned bal = __ballot_sync(0xffffffffu, bit);
+          peers &= bit ? bal : ~bal;
         }
-      if (j < width) out[v * width + j] = Cvt<T, S>::f(acc * scale);
+        const unsigned c = valid ? s.count[w][d] : 0u, before = __popc(peers & lt);
+        __syncwarp();
+        if (valid && before == 0) s.count[w][d] = c + __popc(peers);
+        __syncwarp();
+        at[e] = c + before;
+      }
     }
+    __syncthreads();
+    if (tid < 256) {  // thread = digit: each warp's first place among the block's keys of the digit
+      unsigned c[32], t = 0;
+#pragma unroll
+      for (int v = 0; v < 32; ++v) c[v] = s.count[v][tid];
+#pragma unroll
+      for (int v = 0; v < 32; ++v) {
+        s.count[v][tid] = t;
+        t += c[v];
+      }
+      for (int r = 0; r < kSortRanks; ++r) *cl.map_shared_rank(&s.total[rank][tid], r) = t;
+    }
+    cl.sync();
+    if (tid < 256) {
+      unsigned all = 0, below = 0;
+#pragma unroll
+      for (int r = 0; r < kSortRanks; ++r) {
+        const unsigned t = s.total[r][tid];
+        if (r < (int)rank) below += t;
+        all += t;
+      }
+      unsigned inc = all;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned t = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += t;
+      }
+      if (lane == 31) s.sum[w] = inc;
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      unsigned pre = 0;
+#pragma unroll
+      for (unsigned v = 0; v < 8; ++v)
+        if (v < w) pre += s.sum[v];
+      s.base[tid] = pre + inc - all + below;
+    }
+    __syncthreads();
+    const bool final = pass + 1 == passes;
+    unsigned long long *to = buf[(pass & 1) ^ 1];
+#pragma unroll
+    for (int e = 0; e < kSortItems; ++e) {
+      if (e < items && rank * tile + place + e * 32 < n) {
+        const unsigned d = (unsigned)(k[e] >> shift) & mask;
+        const unsigned dst = s.base[d] + s.count[w][d] + at[e];
+        if (dst >= n) {  // inconsistent counts: report, never write out of bounds
+          atomicExch(err, 4);
+        } else if (final) {
+          keys[dst] = (unsigned)(k[e] >> 32);
+          order[dst] = (unsigned)k[e];
+        } else {
+          const unsigned r = dst / tile;
+          *cl.map_shared_rank(&to[dst - r * tile], r) = k[e];
+        }
+      }
+    }
+    cl.sync();
+  }
+}
+
+// ---- more tokens than a cluster holds: keys for sort_pairs, and the zeros by
+// the sorted keys (a row is written where no key equals it).
+template <class I>
+__global__ void __launch_bounds__(256) emb_prep_kernel(const I *__restrict__ ids, unsigned n, long long rows,
+                                                       long long padding, unsigned *__restrict__ keys,
+                                                       unsigned *__restrict__ order, int *err) {
+  for (unsigned i = blockIdx.x * 256u + threadIdx.x; i < n; i += gridDim.x * 256u) {
+    const long long id = (long long)ids[i];
+    const bool ok = id >= 0 && id < rows;
+    if (!ok) atomicExch(err, 5);
+    keys[i] = (unsigned)(ok && id != padding ? id : rows);
+    order[i] = i;
+  }
+}
+
+template <class T>
+__global__ void __launch_bounds__(256) emb_gaps_kernel(const unsigned *__restrict__ keys, unsigned n, long long rows,
+                                                       FastDiv width, T *__restrict__ out, unsigned bits, int *err) {
+  extern __shared__ unsigned s_seen_raw[];
+  const long long share = (rows + gridDim.x - 1) / gridDim.x;
+  const long long a = share * blockIdx.x, b = a + share < rows ? a + share : rows;
+  for (long long r = a; r < b; r += bits) {
+    const long long e = r + bits < b ? r + bits : b;
+    unsigned lo = 0, hi = n;  // the keys in [r, e)
+    while (lo < hi) {
+      const unsigned mid = lo + (hi - lo) / 2;
+      if (keys[mid] < (unsigned)r) lo = mid + 1;
+      else hi = mid;
+    }
+    const unsigned first = lo;
+    hi = n;
+    while (lo < hi) {
+      const unsigned mid = lo + (hi - lo) / 2;
+      if (keys[mid] < (unsigned)e) lo = mid + 1;
+      else hi = mid;
+    }
+    emb_zero_rows<T, unsigned>(keys + first, lo - first, rows, -1, r, e, width, out, s_seen_raw, err);
+  }
+}
+
+// ---- sums over the sorted tokens.  Shares of `share` tokens; a group of
+// `lanes` threads has one share and the columns of its vectors.  A run of
+// one id inside a share goes to its row; the parts of a run that crosses
+// shares go to part[share][0] (what continues from the share before) and
+// part[share][1] (what begins here and goes on).
+template <class T, int VEC>
+__global__ void __launch_bounds__(256) emb_sum_kernel(const unsigned *__restrict__ keys,
+                                                      const unsigned *__restrict__ order, unsigned n, unsigned share,
+                                                      unsigned shares, unsigned lanes, const T *__restrict__ grad,
+                                                      long long g_stride, unsigned rows, unsigned width,
+                                                      typename EmbAcc<T>::type scale, T *__restrict__ out,
+                                                      typename EmbAcc<T>::type *__restrict__ part) {
+  typedef typename EmbAcc<T>::type S;
+  typedef EmbVec<T, VEC> V;
+  const unsigned grp = threadIdx.x / lanes, groups = 256 / lanes;
+  const unsigned s = blockIdx.x * groups + grp;
+  const unsigned c = (blockIdx.y * lanes + threadIdx.x % lanes) * VEC;
+  if (s >= shares || grp >= groups || c >= width) return;
+  const unsigned i0 = s * share, i1 = n - i0 < share ? n : i0 + share;
+  unsigned cur = keys[i0];
+  if (cur >= rows) return;  // sorted last: nothing from here on counts
+  bool head = i0 > 0 && keys[i0 - 1] == cur;
+  S acc[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) acc[e] = S(0);
+  auto flush = [&](bool on) {
+    if (head || on) {
+      S *p = part + ((size_t)s * 2 + (head ? 0 : 1)) * width + c;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) p[e] = acc[e];
+    } else {
+      V r;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) r.v[e] = Cvt<T, S>::f(acc[e] * scale);
+      *reinterpret_cast<V *>(out + (size_t)cur * width + c) = r;
+    }
+  };
+  constexpr int B = 8;
+  for (unsigned i = i0; i < i1; i += B) {
+    V v[B];
+    unsigned key[B];
+#pragma unroll
+    for (int j = 0; j < B; ++j) {
+      key[j] = i + j < i1 ? keys[i + j] : 0xffffffffu;
+      if (key[j] < rows) v[j] = *reinterpret_cast<const V *>(grad + (long long)order[i + j] * g_stride + c);
+    }
+#pragma unroll
+    for (int j = 0; j < B; ++j) {
+      if (key[j] >= rows) continue;  // past the end, or sorted behind every row
+      if (key[j] != cur) {
+        flush(false);
+        head = false;
+        cur = key[j];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) acc[e] = S(0);
+      }
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) acc[e] += Cvt<S, T>::f(v[j].v[e]);
+    }
+  }
+  flush(i1 < n && keys[i1] == cur);
+}
+
+// Runs that cross shares: the blocks of the share where one begins add its
+// parts, a warp an eighth of them (in order), then the warps' sums in order.
+template <class T, int JV>
+__global__ void __launch_bounds__(256) emb_join_kernel(const unsigned *__restrict__ keys, unsigned n, unsigned share,
+                                                       unsigned rows, unsigned width, typename EmbAcc<T>::type scale,
+                                                       const typename EmbAcc<T>::type *__restrict__ part,
+                                                       T *__restrict__ out) {
+  typedef typename EmbAcc<T>::type S;
+  typedef EmbVec<S, JV> V;
+  __shared__ V s_part[8][32];
+  const unsigned s = blockIdx.x, i0 = s * share, i1 = n - i0 < share ? n : i0 + share;
+  const unsigned key = keys[i1 - 1];
+  if (key >= rows || i1 == n || keys[i1] != key) return;         // no run goes on from here
+  if (i0 > 0 && keys[i0] == key && keys[i0 - 1] == key) return;  // it began earlier
+  unsigned lo = i1, hi = n;                                      // where it ends
+  while (lo < hi) {
+    const unsigned mid = lo + (hi - lo) / 2;
+    if (keys[mid] <= key) lo = mid + 1;
+    else hi = mid;
+  }
+  const unsigned more = (lo - 1) / share - s;  // shares that continue it
+  const unsigned lane = threadIdx.x & 31, w = threadIdx.x >> 5, eighth = (more + 7) / 8;
+  const unsigned a = s + 1 + w * eighth, b = a + eighth < s + 1 + more ? a + eighth : s + 1 + more;
+  for (unsigned c0 = blockIdx.y * 32 * JV; c0 < width; c0 += gridDim.y * 32 * JV) {
+    const unsigned c = c0 + lane * JV;
+    V acc;
+#pragma unroll
+    for (int e = 0; e < JV; ++e) acc.v[e] = S(0);
+    if (c < width) {
+      if (w == 0) acc = *reinterpret_cast<const V *>(part + ((size_t)s * 2 + 1) * width + c);
+#pragma unroll 8
+      for (unsigned t = a; t < b; ++t) {
+        const V v = *reinterpret_cast<const V *>(part + (size_t)t * 2 * width + c);
+#pragma unroll
+        for (int e = 0; e < JV; ++e) acc.v[e] += v.v[e];
+      }
+    }
+    s_part[w][lane] = acc;
+    __syncthreads();
+    if (w == 0 && c < width) {
+      for (int v = 1; v < 8; ++v)
+#pragma unroll
+        for (int e = 0; e < JV; ++e) acc.v[e] += s_part[v][lane].v[e];
+#pragma unroll
+      for (int e = 0; e < JV; ++e) out[(size_t)key * width + c + e] = Cvt<T, S>::f(acc.v[e] * scale);
+    }
+    __syncthreads();
   }
 }
 
@@ -66,40 +511,190 @@ __global__ void __launch_bounds__(256) emb_grad_kernel(const I *__restrict__ ids
 
 namespace {
 
+using mmpd::FastDiv;
+
+FastDiv emb_div(unsigned d) {
+  unsigned l = 0;
+  while (l < 32 && (1ull << l) < d) ++l;
+  FastDiv f;
+  f.d = d;
+  f.m = (unsigned)(((1ull << 32) * ((1ull << l) - d)) / d + 1);
+  f.s = l;
+  return f;
+}
+
 int emb_check(const char *what, int dtype, int ids_dtype, int64_t rows, int64_t width, int64_t n) {
   if (rows < 0 || width < 0 || n < 0) return mmp::set_error(MMP_E_ARG, std::string(what) + ": negative size");
   if (dtype != MMP_FLOAT16 && dtype != MMP_FLOAT32 && dtype != MMP_FLOAT64)
     return mmp::set_error(MMP_E_ARG, std::string(what) + ": needs a floating dtype");
   if (ids_dtype != MMP_INT32 && ids_dtype != MMP_INT64)
     return mmp::set_error(MMP_E_ARG, std::string(what) + ": ids must be int32 or int64");
-  if (rows > INT32_MAX || n > INT32_MAX || width > INT32_MAX)
-    return mmp::set_error(MMP_E_ARG, std::string(what) + ": a size passes 2^31 - 1");
+  if (rows > (1 << 30) || n > (1 << 30) || width > (1 << 30))
+    return mmp::set_error(MMP_E_ARG, std::string(what) + ": a size passes 2^30");
   return MMP_OK;
 }
 
-unsigned emb_grid(long long want) {
-  const long long cap = (long long)mmp::sm_count() * 16;
-  return (unsigned)(want < cap ? want : cap);
+// Elements that every row can be moved in at once: 16 bytes where width,
+// strides and pointers allow it, 4 bytes for float16 in rows of even width,
+// else one.
+template <class T> int emb_vec(const void *p, const void *q, long long width, long long stride) {
+  for (int bytes = 16; bytes > (int)sizeof(T); bytes = bytes == 16 && sizeof(T) == 2 ? 4 : (int)sizeof(T)) {
+    const int vec = bytes / (int)sizeof(T);
+    if ((uintptr_t)p % bytes == 0 && (uintptr_t)q % bytes == 0 && width % vec == 0 && stride % vec == 0) return vec;
+  }
+  return 1;
+}
+
+template <class T, class I, int VEC>
+int emb_launch(const T *w, int64_t rows, int64_t width, int64_t w_stride, const I *ids, int64_t n, double scale,
+               T *out) {
+  typedef typename mmpd::EmbAcc<T>::type S;
+  const int64_t per = width / VEC;
+  // in parts whose vectors 32 bits count
+  const int64_t most = (INT64_C(1) << 31) / per > 0 ? (INT64_C(1) << 31) / per : 1;
+  for (int64_t r = 0; r < n; r += most) {
+    const int64_t m = n - r < most ? n - r : most;
+    const unsigned total = (unsigned)(m * per);
+    int *err = mmp::device_error_word();
+    // four vectors a thread where that leaves every SM its blocks
+    if (total >= 1024u * 4 * (unsigned)mmp::sm_count())
+      mmpd::emb_kernel<T, I, VEC, 4><<<(total + 1023) / 1024, 256, 0, mmp::stream()>>>(
+          w, rows, emb_div((unsigned)per), w_stride, ids + r, total, (S)scale, out + r * width, err);
+    else
+      mmpd::emb_kernel<T, I, VEC, 1><<<(total + 255) / 256, 256, 0, mmp::stream()>>>(
+          w, rows, emb_div((unsigned)per), w_stride, ids + r, total, (S)scale, out + r * width, err);
+    MMP_LAUNCH_CHECK("embedding");
+  }
+  return MMP_OK;
 }
 
 template <class T, class I>
 int run_emb(const void *w, int64_t rows, int64_t width, int64_t w_stride, const void *ids, int64_t n, double scale,
             void *out) {
-  mmpd::emb_kernel<T, I><<<emb_grid(n), 256, 0, mmp::stream()>>>((const T *)w, rows, width, w_stride, (const I *)ids,
-                                                               n, (typename mmpd::EmbAcc<T>::type)scale, (T *)out,
-                                                               mmp::device_error_word());
-  MMP_LAUNCH_CHECK("embedding");
+  const int vec = emb_vec<T>(w, out, width, w_stride);
+  if (vec * sizeof(T) == 16)
+    return emb_launch<T, I, 16 / (int)sizeof(T)>((const T *)w, rows, width, w_stride, (const I *)ids, n, scale, (T *)out);
+  if constexpr (sizeof(T) == 2)
+    if (vec == 2) return emb_launch<T, I, 2>((const T *)w, rows, width, w_stride, (const I *)ids, n, scale, (T *)out);
+  return emb_launch<T, I, 1>((const T *)w, rows, width, w_stride, (const I *)ids, n, scale, (T *)out);
+}
+
+// Device memory of one call, from the stream-ordered pool.
+struct EmbBuf {
+  void *p = nullptr;
+  int alloc(size_t bytes) {
+    MMP_CUDA_TRY(cudaMallocAsync(&p, bytes, mmp::stream()));
+    return MMP_OK;
+  }
+  ~EmbBuf() {
+    if (p) cudaFreeAsync(p, mmp::stream());
+  }
+};
+
+template <class T, class I, int VEC>
+int emb_few(const I *ids, unsigned n, const T *grad, int64_t g_stride, int64_t rows, int64_t width, double scale,
+            int64_t padding, T *out) {
+  // a block a token, and eight an SM for the zeros while they have a 64 KB each
+  const int64_t most = (int64_t)mmp::sm_count() * 8, want = rows * width * (int64_t)sizeof(T) / 65536 + 1;
+  const unsigned zero = (unsigned)(want < most ? want : most);
+  mmpd::emb_grad_few<T, I, VEC><<<n + zero, 256, 0, mmp::stream()>>>(
+      ids, n, grad, g_stride, rows, emb_div((unsigned)width), (typename mmpd::EmbAcc<T>::type)scale, padding, out,
+      mmp::device_error_word());
+  MMP_LAUNCH_CHECK("embedding_grad");
+  return MMP_OK;
+}
+
+template <class T, class I, int VEC>
+int emb_sum(const unsigned *keys, const unsigned *order, unsigned n, const T *grad, int64_t g_stride, int64_t rows,
+            int64_t width, double scale, T *out) {
+  typedef typename mmpd::EmbAcc<T>::type S;
+  unsigned lanes = 1;
+  while (lanes < 256 && lanes * VEC < width) lanes *= 2;
+  const unsigned slices = (unsigned)((width + (int64_t)lanes * VEC - 1) / ((int64_t)lanes * VEC)), groups = 256 / lanes;
+  // shares of 32 tokens: fewer where that leaves SMs without blocks, more
+  // where it makes more than sixteen blocks an SM (each share may leave two
+  // parts to join)
+  unsigned share = 32;
+  auto blocks = [&] { return ((uint64_t)n + share - 1) / share * slices / groups; };
+  while (share > 8 && blocks() < 4u * (unsigned)mmp::sm_count()) share /= 2;
+  while (blocks() > 16u * (unsigned)mmp::sm_count()) share *= 2;
+  const unsigned shares = (n + share - 1) / share;
+  EmbBuf part;
+  const int rc = part.alloc((size_t)shares * 2 * width * sizeof(S));
+  if (rc) return rc;
+  mmpd::emb_sum_kernel<T, VEC><<<dim3((shares + groups - 1) / groups, slices), 256, 0, mmp::stream()>>>(
+      keys, order, n, share, shares, lanes, grad, g_stride, (unsigned)rows, (unsigned)width, (S)scale, out, (S *)part.p);
+  MMP_LAUNCH_CHECK("embedding_grad sums");
+  constexpr int JV = VEC >= 4 ? 4 : 1;
+  const unsigned cols = (unsigned)((width + 32 * JV - 1) / (32 * JV));
+  mmpd::emb_join_kernel<T, JV><<<dim3(shares, cols < 32 ? cols : 32), 256, 0, mmp::stream()>>>(
+      keys, n, share, (unsigned)rows, (unsigned)width, (S)scale, (const S *)part.p, out);
+  MMP_LAUNCH_CHECK("embedding_grad join");
   return MMP_OK;
 }
 
 template <class T, class I>
-int run_emb_grad(const void *ids, int64_t n, const void *grad, int64_t g_stride, int64_t rows, int64_t width,
-                 double scale, int64_t padding, void *out) {
-  mmpd::emb_grad_kernel<T, I><<<emb_grid((rows + 7) / 8), 256, 0, mmp::stream()>>>(
-      (const I *)ids, n, (const T *)grad, g_stride, rows, width, (typename mmpd::EmbAcc<T>::type)scale, padding,
-      (T *)out, mmp::device_error_word());
-  MMP_LAUNCH_CHECK("embedding_grad");
-  return MMP_OK;
+int run_emb_grad(const void *ids_, int64_t n, const void *grad_, int64_t g_stride, int64_t rows, int64_t width,
+                 double scale, int64_t padding, void *out_) {
+  const I *ids = (const I *)ids_;
+  const T *grad = (const T *)grad_;
+  T *out = (T *)out_;
+  const int vec = emb_vec<T>(grad, out, width, g_stride);
+  constexpr int WIDE = 16 / (int)sizeof(T);
+  if (n <= mmpd::kEmbFew) {
+    if (vec == WIDE) return emb_few<T, I, WIDE>(ids, (unsigned)n, grad, g_stride, rows, width, scale, padding, out);
+    if constexpr (sizeof(T) == 2)
+      if (vec == 2) return emb_few<T, I, 2>(ids, (unsigned)n, grad, g_stride, rows, width, scale, padding, out);
+    return emb_few<T, I, 1>(ids, (unsigned)n, grad, g_stride, rows, width, scale, padding, out);
+  }
+  int bits = 1;
+  while ((INT64_C(1) << bits) <= rows) ++bits;  // the key `rows` included
+  const FastDiv wd = emb_div((unsigned)width);
+  int *err = mmp::device_error_word();
+  EmbBuf mem;
+  const size_t np = ((size_t)n + 3) & ~(size_t)3;
+  unsigned *keys, *order;
+  if (n <= mmpd::kEmbCluster) {
+    int rc = mem.alloc(np * 8);
+    if (rc) return rc;
+    keys = (unsigned *)mem.p;
+    order = keys + np;
+    const int items = (int)((n + mmpd::kSortThreads * mmpd::kSortRanks - 1) / (mmpd::kSortThreads * mmpd::kSortRanks));
+    const int passes = (bits + 7) / 8, digit = (bits + passes - 1) / passes;
+    // one block an SM; clusters of eight fill 16 SMs of each of the GPU's parts
+    const int64_t most = mmp::sm_count() / mmpd::kSortRanks - 1;
+    const int64_t want = rows * width * (int64_t)sizeof(T) / (65536 * mmpd::kSortRanks) + 1;
+    const unsigned clusters = 1 + (unsigned)(want < most ? want : most);
+    const int64_t share = (rows + (clusters - 1) * mmpd::kSortRanks - 1) / ((clusters - 1) * mmpd::kSortRanks);
+    size_t smem = sizeof(mmpd::EmbSortSmem) + (size_t)items * mmpd::kSortThreads * 16;
+    const size_t seen = (size_t)(share < 524288 ? (share + 31) / 32 * 4 : 65536);
+    if (smem < seen) smem = seen;
+    auto fn = mmpd::emb_sort_kernel<T, I>;
+    MMP_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    fn<<<clusters * mmpd::kSortRanks, mmpd::kSortThreads, smem, mmp::stream()>>>(
+        ids, (unsigned)n, rows, padding, items, passes, digit, keys, order, wd, out, (unsigned)(seen * 8), err);
+    MMP_LAUNCH_CHECK("embedding_grad sort");
+  } else {
+    int rc = mem.alloc(np * 16);
+    if (rc) return rc;
+    unsigned *const kb[2] = {(unsigned *)mem.p, (unsigned *)mem.p + np};
+    unsigned *const ob[2] = {kb[1] + np, kb[1] + 2 * np};
+    mmpd::emb_prep_kernel<I><<<mmp::sm_count() * 8, 256, 0, mmp::stream()>>>(ids, (unsigned)n, rows, padding, kb[0],
+                                                                             ob[0], err);
+    MMP_LAUNCH_CHECK("embedding_grad keys");
+    int cur = 0;
+    rc = mmp::sort_pairs(kb, ob, (unsigned)n, bits, &cur);
+    if (rc) return rc;
+    keys = kb[cur];
+    order = ob[cur];
+    const unsigned blocks = (unsigned)mmp::sm_count() * 8;
+    mmpd::emb_gaps_kernel<T><<<blocks, 256, 16384, mmp::stream()>>>(keys, (unsigned)n, rows, wd, out, 131072u, err);
+    MMP_LAUNCH_CHECK("embedding_grad zeros");
+  }
+  if (vec == WIDE) return emb_sum<T, I, WIDE>(keys, order, (unsigned)n, grad, g_stride, rows, width, scale, out);
+  if constexpr (sizeof(T) == 2)
+    if (vec == 2) return emb_sum<T, I, 2>(keys, order, (unsigned)n, grad, g_stride, rows, width, scale, out);
+  return emb_sum<T, I, 1>(keys, order, (unsigned)n, grad, g_stride, rows, width, scale, out);
 }
 
 }  // namespace

@@ -36,6 +36,10 @@ bool peer_table(void **blk, int *rank, int *nranks, unsigned long long *epoch);
 int scan_carry_allranks(int prod, int dtype, const void *agg, long long ntiles, const void *x, long long n,
                         void *carry_out);
 
+// Stable asynchronous sort of n keys below 2^bits with their payload between
+// two buffers each; *cur: the one that holds the result (mmp_sort.cu).
+int sort_pairs(unsigned *const keys[2], unsigned *const payload[2], unsigned n, int bits, int *cur);
+
 }  // namespace mmp
 
 #define MMP_CUDA_TRY(call)                                   \
