@@ -74,13 +74,30 @@ __global__ void __launch_bounds__(256) emb_kernel(const T *__restrict__ w, long 
   }
 }
 
+// Zeros to `n` elements by one warp: 16-byte pieces, the ends element by
+// element.
+template <class T> __device__ __forceinline__ void emb_zero(T *p, long long n) {
+  constexpr int PE = 16 / (int)sizeof(T);
+  const T zero = Cvt<T, float>::f(0.0f);
+  const int lane = threadIdx.x & 31;
+  long long head = (long long)((16 - ((uintptr_t)p & 15)) & 15) / (long long)sizeof(T);
+  if (head > n) head = n;
+  if (lane < head) p[lane] = zero;  // at most 7
+  p += head;
+  n -= head;
+  uint4 *q = reinterpret_cast<uint4 *>(p);
+  const long long pieces = n / PE;
+#pragma unroll 4
+  for (long long i = lane; i < pieces; i += 32) q[i] = make_uint4(0, 0, 0, 0);
+  if (lane < n - pieces * PE) p[pieces * PE + lane] = zero;
+}
+
 // ---- zeros of the rows [r0, r1) that no token has, by one block.  s_seen: a
-// bitmap of at least r1 - r0 bits.  The rows are one stretch of memory,
-// written in 16-byte pieces; a piece that belongs to two rows, or sticks out
-// at an end, goes element by element.
+// bitmap of at least r1 - r0 bits.  A warp takes `unit` rows of one word of
+// it; neighbouring rows without a token are one stretch of memory.
 template <class T, class I>
 __device__ void emb_zero_rows(const I *__restrict__ ids, unsigned n, long long rows, long long padding, long long r0,
-                              long long r1, FastDiv width, T *__restrict__ out, unsigned *s_seen, int *err) {
+                              long long r1, unsigned width, T *__restrict__ out, unsigned *s_seen, int *err) {
   const unsigned tid = threadIdx.x, nt = blockDim.x;
   const unsigned count = (unsigned)(r1 - r0);
   __syncthreads();
@@ -93,42 +110,25 @@ __device__ void emb_zero_rows(const I *__restrict__ ids, unsigned n, long long r
     if (r0 == 0 && (id < 0 || id >= rows)) atomicExch(err, 5);
   }
   __syncthreads();
-  auto seen = [&](unsigned r) { return (s_seen[r >> 5] >> (r & 31)) & 1u; };
-  // in parts of rows whose elements 32 bits count
-  const unsigned part = 0x7fffffffu / width.d > count ? count : 0x7fffffffu / width.d ? 0x7fffffffu / width.d : 1;
-  constexpr unsigned PE = 16 / sizeof(T);
-  const T zero = Cvt<T, float>::f(0.0f);
-  for (unsigned p0 = 0; p0 < count; p0 += part) {
-    T *base = out + (r0 + p0) * width.d;
-    const unsigned elems = (count - p0 < part ? count - p0 : part) * width.d;
-    const unsigned head = (unsigned)((16 - ((uintptr_t)base & 15)) & 15) / (unsigned)sizeof(T);
-    const unsigned pieces = elems > head ? (elems - head) / PE : 0;
-    const unsigned tail = elems > head ? head + pieces * PE : 0;  // elements outside: [0, head) and [tail, elems)
-    for (unsigned i = tid; i < pieces; i += nt) {
-      const unsigned e = head + i * PE;
-      const unsigned ra = width.div(e), rb = width.div(e + PE - 1);
-      bool a = seen(p0 + ra), b = seen(p0 + rb);
-      if (rb > ra + 1) a = true;  // rows shorter than a piece
-      if (!a && !b) {
-        *reinterpret_cast<uint4 *>(base + e) = make_uint4(0, 0, 0, 0);
-      } else if (ra != rb) {
-        for (unsigned j = 0; j < PE; ++j)
-          if (!seen(p0 + width.div(e + j))) base[e + j] = zero;
-      }
+  // four units a warp at least, where there are rows enough
+  unsigned unit = 32;
+  while (unit > 1 && count / unit < nt / 32 * 4) unit /= 2;
+  for (unsigned r = tid / 32 * unit; r < count; r += nt / 32 * unit) {
+    const unsigned m = count - r < unit ? count - r : unit;
+    unsigned open = ~(s_seen[r >> 5] >> (r & 31)) & (m == 32 ? 0xffffffffu : (1u << m) - 1);
+    while (open) {
+      const unsigned lo = __ffs(open) - 1, over = ~(open >> lo);
+      const unsigned len = over ? __ffs(over) - 1 : 32;
+      emb_zero(out + (r0 + r + lo) * width, (long long)len * width);
+      open &= len == 32 ? 0u : ~(((1u << len) - 1) << lo);
     }
-    const unsigned h = head < elems ? head : elems;
-    for (unsigned e = tid; e < h; e += nt)
-      if (!seen(p0 + width.div(e))) base[e] = zero;
-    if (elems > head)
-      for (unsigned e = tail + tid; e < elems; e += nt)
-        if (!seen(p0 + width.div(e))) base[e] = zero;
   }
 }
 
 // This block's part of the rows, in stretches of at most `bits` rows.
 template <class T, class I>
 __device__ __forceinline__ void emb_zero_share(const I *ids, unsigned n, long long rows, long long padding, unsigned part,
-                                               unsigned parts, unsigned bits, FastDiv width, T *out, unsigned *s_seen,
+                                               unsigned parts, unsigned bits, unsigned width, T *out, unsigned *s_seen,
                                                int *err) {
   const long long share = (rows + parts - 1) / parts;
   const long long a = share * part, b = a + share < rows ? a + share : rows;
@@ -143,7 +143,7 @@ constexpr unsigned kEmbFewBits = 16384;  // rows a block of that path marks at o
 // first of its id, adds all of them in the order of n.  The others: zeros.
 template <class T, class I, int VEC>
 __global__ void __launch_bounds__(256) emb_grad_few(const I *__restrict__ ids, unsigned n, const T *__restrict__ grad,
-                                                    long long g_stride, long long rows, FastDiv width,
+                                                    long long g_stride, long long rows, unsigned width,
                                                     typename EmbAcc<T>::type scale, long long padding,
                                                     T *__restrict__ out, int *err) {
   typedef typename EmbAcc<T>::type S;
@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(256) emb_grad_few(const I *__restrict__ ids, u
   for (unsigned u = 0; u < kEmbFew / 256; ++u)
     if (hit >> u & 1) s_buf[before++] = tid * (kEmbFew / 256) + u;
   __syncthreads();
-  for (unsigned c = tid * VEC; c < width.d; c += 256 * VEC) {
+  for (unsigned c = tid * VEC; c < width; c += 256 * VEC) {
     S acc[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) acc[e] = S(0);
@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(256) emb_grad_few(const I *__restrict__ ids, u
     V r;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) r.v[e] = Cvt<T, S>::f(acc[e] * scale);
-    *reinterpret_cast<V *>(out + id * width.d + c) = r;
+    *reinterpret_cast<V *>(out + id * width + c) = r;
   }
 }
 
@@ -244,8 +244,8 @@ __device__ __forceinline__ unsigned emb_lanemask_lt() {
 template <class T, class I>
 __global__ void __cluster_dims__(kSortRanks, 1, 1) __launch_bounds__(kSortThreads, 1)
     emb_sort_kernel(const I *__restrict__ ids, unsigned n, long long rows, long long padding, int items, int passes,
-                    int digit, unsigned *__restrict__ keys, unsigned *__restrict__ order, FastDiv width,
-                    T *__restrict__ out, unsigned bits, int *err) {
+                    int digit, unsigned *__restrict__ keys, unsigned *__restrict__ order, unsigned width,
+                    T *__restrict__ out, unsigned bits, unsigned *__restrict__ runs, int *err) {
   extern __shared__ __align__(16) unsigned char s_raw[];
   if (blockIdx.x >= kSortRanks) {
     emb_zero_share<T, I>(ids, n, rows, padding, blockIdx.x - kSortRanks, gridDim.x - kSortRanks, bits, width, out,
@@ -258,6 +258,7 @@ __global__ void __cluster_dims__(kSortRanks, 1, 1) __launch_bounds__(kSortThread
   const unsigned tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const unsigned tile = items * kSortThreads;
   unsigned long long *const buf[2] = {s.key[0], s.key[0] + tile};
+  if (rank == 0 && tid == 0) *runs = 0;
   const unsigned place = w * items * 32 + lane;  // this thread's keys: place + 32 e
   const unsigned lt = emb_lanemask_lt();
   for (int e = 0; e < items; ++e) {
@@ -371,8 +372,10 @@ __global__ void __launch_bounds__(256) emb_prep_kernel(const I *__restrict__ ids
 
 template <class T>
 __global__ void __launch_bounds__(256) emb_gaps_kernel(const unsigned *__restrict__ keys, unsigned n, long long rows,
-                                                       FastDiv width, T *__restrict__ out, unsigned bits, int *err) {
+                                                       unsigned width, T *__restrict__ out, unsigned bits,
+                                                       unsigned *__restrict__ runs, int *err) {
   extern __shared__ unsigned s_seen_raw[];
+  if (blockIdx.x == 0 && threadIdx.x == 0) *runs = 0;
   const long long share = (rows + gridDim.x - 1) / gridDim.x;
   const long long a = share * blockIdx.x, b = a + share < rows ? a + share : rows;
   for (long long r = a; r < b; r += bits) {
@@ -395,27 +398,45 @@ __global__ void __launch_bounds__(256) emb_gaps_kernel(const unsigned *__restric
 }
 
 // ---- sums over the sorted tokens.  Shares of `share` tokens; a group of
-// `lanes` threads has one share and the columns of its vectors.  A run of
-// one id inside a share goes to its row; the parts of a run that crosses
-// shares go to part[share][0] (what continues from the share before) and
-// part[share][1] (what begins here and goes on).
+// `lanes` threads has one share and the columns of its vectors.  The share
+// where a run of one id begins adds it whole, into the next share if it ends
+// there.  A run of further shares is left in parts, part[share][0] (what
+// continues from the share before) and part[share][1] (what begins here),
+// and listed in `list` for the next kernel (in any order).
 template <class T, int VEC>
 __global__ void __launch_bounds__(256) emb_sum_kernel(const unsigned *__restrict__ keys,
                                                       const unsigned *__restrict__ order, unsigned n, unsigned share,
                                                       unsigned shares, unsigned lanes, const T *__restrict__ grad,
                                                       long long g_stride, unsigned rows, unsigned width,
                                                       typename EmbAcc<T>::type scale, T *__restrict__ out,
-                                                      typename EmbAcc<T>::type *__restrict__ part) {
+                                                      typename EmbAcc<T>::type *__restrict__ part,
+                                                      unsigned *__restrict__ runs, unsigned *__restrict__ list) {
   typedef typename EmbAcc<T>::type S;
   typedef EmbVec<T, VEC> V;
   const unsigned grp = threadIdx.x / lanes, groups = 256 / lanes;
   const unsigned s = blockIdx.x * groups + grp;
   const unsigned c = (blockIdx.y * lanes + threadIdx.x % lanes) * VEC;
   if (s >= shares || grp >= groups || c >= width) return;
-  const unsigned i0 = s * share, i1 = n - i0 < share ? n : i0 + share;
-  unsigned cur = keys[i0];
+  unsigned i = s * share;
+  const unsigned i0 = i, i1 = n - i < share ? n : i + share;
+  unsigned cur = keys[i];
   if (cur >= rows) return;  // sorted last: nothing from here on counts
-  bool head = i0 > 0 && keys[i0 - 1] == cur;
+  bool head = i > 0 && keys[i - 1] == cur;
+  if (head && (i == share || keys[i - share - 1] != cur) && (i1 == n || keys[i1] != cur)) {
+    // the share before has this run
+    head = false;
+    while (i < i1 && keys[i] == cur) ++i;
+    if (i == i1) return;
+    cur = keys[i];
+    if (cur >= rows) return;
+  }
+  // the last run: to its end if that lies in the next share
+  const unsigned after = i1 < n ? keys[i1] : rows;  // a key that goes on behind this share
+  const bool goes = after < rows && keys[i1 - 1] == after;
+  // (a run that comes from the share before and goes on is longer than that)
+  const bool from = goes && keys[i0] == after && i0 > 0 && keys[i0 - 1] == after;
+  const bool far = goes && (from || (i1 + share < n && keys[i1 + share] == after));
+  const unsigned stop = goes && !far ? (i1 + share < n ? i1 + share : n) : i1;
   S acc[VEC];
 #pragma unroll
   for (int e = 0; e < VEC; ++e) acc[e] = S(0);
@@ -424,6 +445,7 @@ __global__ void __launch_bounds__(256) emb_sum_kernel(const unsigned *__restrict
       S *p = part + ((size_t)s * 2 + (head ? 0 : 1)) * width + c;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) p[e] = acc[e];
+      if (!head && c == 0) list[atomicAdd(runs, 1u)] = s;
     } else {
       V r;
 #pragma unroll
@@ -432,12 +454,13 @@ __global__ void __launch_bounds__(256) emb_sum_kernel(const unsigned *__restrict
     }
   };
   constexpr int B = 8;
-  for (unsigned i = i0; i < i1; i += B) {
+  for (; i < stop; i += B) {
     V v[B];
     unsigned key[B];
 #pragma unroll
     for (int j = 0; j < B; ++j) {
-      key[j] = i + j < i1 ? keys[i + j] : 0xffffffffu;
+      key[j] = i + j < stop ? keys[i + j] : rows;
+      if (i + j >= i1 && key[j] != after) key[j] = rows;  // the next share's own
       if (key[j] < rows) v[j] = *reinterpret_cast<const V *>(grad + (long long)order[i + j] * g_stride + c);
     }
 #pragma unroll
@@ -454,56 +477,59 @@ __global__ void __launch_bounds__(256) emb_sum_kernel(const unsigned *__restrict
       for (int e = 0; e < VEC; ++e) acc[e] += Cvt<S, T>::f(v[j].v[e]);
     }
   }
-  flush(i1 < n && keys[i1] == cur);
+  flush(far);
 }
 
-// Runs that cross shares: the blocks of the share where one begins add its
-// parts, a warp an eighth of them (in order), then the warps' sums in order.
+// Listed runs: the parts of one in order, a warp an eighth of them, then the
+// warps' sums in order.
 template <class T, int JV>
 __global__ void __launch_bounds__(256) emb_join_kernel(const unsigned *__restrict__ keys, unsigned n, unsigned share,
-                                                       unsigned rows, unsigned width, typename EmbAcc<T>::type scale,
+                                                       unsigned width, typename EmbAcc<T>::type scale,
                                                        const typename EmbAcc<T>::type *__restrict__ part,
-                                                       T *__restrict__ out) {
+                                                       const unsigned *__restrict__ runs,
+                                                       const unsigned *__restrict__ list, T *__restrict__ out) {
   typedef typename EmbAcc<T>::type S;
   typedef EmbVec<S, JV> V;
   __shared__ V s_part[8][32];
-  const unsigned s = blockIdx.x, i0 = s * share, i1 = n - i0 < share ? n : i0 + share;
-  const unsigned key = keys[i1 - 1];
-  if (key >= rows || i1 == n || keys[i1] != key) return;         // no run goes on from here
-  if (i0 > 0 && keys[i0] == key && keys[i0 - 1] == key) return;  // it began earlier
-  unsigned lo = i1, hi = n;                                      // where it ends
-  while (lo < hi) {
-    const unsigned mid = lo + (hi - lo) / 2;
-    if (keys[mid] <= key) lo = mid + 1;
-    else hi = mid;
-  }
-  const unsigned more = (lo - 1) / share - s;  // shares that continue it
-  const unsigned lane = threadIdx.x & 31, w = threadIdx.x >> 5, eighth = (more + 7) / 8;
-  const unsigned a = s + 1 + w * eighth, b = a + eighth < s + 1 + more ? a + eighth : s + 1 + more;
-  for (unsigned c0 = blockIdx.y * 32 * JV; c0 < width; c0 += gridDim.y * 32 * JV) {
-    const unsigned c = c0 + lane * JV;
-    V acc;
+  const unsigned lane = threadIdx.x & 31, w = threadIdx.x >> 5, count = *runs;
+  for (unsigned k = blockIdx.x; k < count; k += gridDim.x) {
+    const unsigned s = list[k], i1 = (s + 1) * share, key = keys[i1];
+    // the run ends in share s + more: doubling steps, then halving
+    unsigned step = 2;
+    while ((s + step) * (unsigned long long)share < n && keys[(s + step) * share] == key) step *= 2;
+    unsigned lo = step / 2, hi = step;  // share s + lo begins with the key, s + hi does not
+    while (lo + 1 < hi) {
+      const unsigned mid = lo + (hi - lo) / 2;
+      if ((s + mid) * (unsigned long long)share < n && keys[(s + mid) * share] == key) lo = mid;
+      else hi = mid;
+    }
+    const unsigned more = lo, eighth = (more + 7) / 8;
+    const unsigned a = s + 1 + w * eighth, b = a + eighth < s + 1 + more ? a + eighth : s + 1 + more;
+    for (unsigned c0 = blockIdx.y * 32 * JV; c0 < width; c0 += gridDim.y * 32 * JV) {
+      const unsigned c = c0 + lane * JV;
+      V acc;
 #pragma unroll
-    for (int e = 0; e < JV; ++e) acc.v[e] = S(0);
-    if (c < width) {
-      if (w == 0) acc = *reinterpret_cast<const V *>(part + ((size_t)s * 2 + 1) * width + c);
+      for (int e = 0; e < JV; ++e) acc.v[e] = S(0);
+      if (c < width) {
+        if (w == 0) acc = *reinterpret_cast<const V *>(part + ((size_t)s * 2 + 1) * width + c);
 #pragma unroll 8
-      for (unsigned t = a; t < b; ++t) {
-        const V v = *reinterpret_cast<const V *>(part + (size_t)t * 2 * width + c);
+        for (unsigned t = a; t < b; ++t) {
+          const V v = *reinterpret_cast<const V *>(part + (size_t)t * 2 * width + c);
 #pragma unroll
-        for (int e = 0; e < JV; ++e) acc.v[e] += v.v[e];
+          for (int e = 0; e < JV; ++e) acc.v[e] += v.v[e];
+        }
       }
-    }
-    s_part[w][lane] = acc;
-    __syncthreads();
-    if (w == 0 && c < width) {
-      for (int v = 1; v < 8; ++v)
+      s_part[w][lane] = acc;
+      __syncthreads();
+      if (w == 0 && c < width) {
+        for (int v = 1; v < 8; ++v)
 #pragma unroll
-        for (int e = 0; e < JV; ++e) acc.v[e] += s_part[v][lane].v[e];
+          for (int e = 0; e < JV; ++e) acc.v[e] += s_part[v][lane].v[e];
 #pragma unroll
-      for (int e = 0; e < JV; ++e) out[(size_t)key * width + c + e] = Cvt<T, S>::f(acc.v[e] * scale);
+        for (int e = 0; e < JV; ++e) out[(size_t)key * width + c + e] = Cvt<T, S>::f(acc.v[e] * scale);
+      }
+      __syncthreads();
     }
-    __syncthreads();
   }
 }
 
@@ -598,15 +624,15 @@ int emb_few(const I *ids, unsigned n, const T *grad, int64_t g_stride, int64_t r
   const int64_t most = (int64_t)mmp::sm_count() * 8, want = rows * width * (int64_t)sizeof(T) / 65536 + 1;
   const unsigned zero = (unsigned)(want < most ? want : most);
   mmpd::emb_grad_few<T, I, VEC><<<n + zero, 256, 0, mmp::stream()>>>(
-      ids, n, grad, g_stride, rows, emb_div((unsigned)width), (typename mmpd::EmbAcc<T>::type)scale, padding, out,
+      ids, n, grad, g_stride, rows, (unsigned)width, (typename mmpd::EmbAcc<T>::type)scale, padding, out,
       mmp::device_error_word());
   MMP_LAUNCH_CHECK("embedding_grad");
   return MMP_OK;
 }
 
 template <class T, class I, int VEC>
-int emb_sum(const unsigned *keys, const unsigned *order, unsigned n, const T *grad, int64_t g_stride, int64_t rows,
-            int64_t width, double scale, T *out) {
+int emb_sum(const unsigned *keys, const unsigned *order, unsigned *runs, unsigned n, const T *grad, int64_t g_stride,
+            int64_t rows, int64_t width, double scale, T *out) {
   typedef typename mmpd::EmbAcc<T>::type S;
   unsigned lanes = 1;
   while (lanes < 256 && lanes * VEC < width) lanes *= 2;
@@ -620,15 +646,18 @@ int emb_sum(const unsigned *keys, const unsigned *order, unsigned n, const T *gr
   while (blocks() > 16u * (unsigned)mmp::sm_count()) share *= 2;
   const unsigned shares = (n + share - 1) / share;
   EmbBuf part;
-  const int rc = part.alloc((size_t)shares * 2 * width * sizeof(S));
+  const size_t np = (size_t)shares * 2 * width * sizeof(S);
+  const int rc = part.alloc(np + shares * 4);
   if (rc) return rc;
+  unsigned *list = (unsigned *)((char *)part.p + np);
   mmpd::emb_sum_kernel<T, VEC><<<dim3((shares + groups - 1) / groups, slices), 256, 0, mmp::stream()>>>(
-      keys, order, n, share, shares, lanes, grad, g_stride, (unsigned)rows, (unsigned)width, (S)scale, out, (S *)part.p);
+      keys, order, n, share, shares, lanes, grad, g_stride, (unsigned)rows, (unsigned)width, (S)scale, out, (S *)part.p,
+      runs, list);
   MMP_LAUNCH_CHECK("embedding_grad sums");
   constexpr int JV = VEC >= 4 ? 4 : 1;
   const unsigned cols = (unsigned)((width + 32 * JV - 1) / (32 * JV));
-  mmpd::emb_join_kernel<T, JV><<<dim3(shares, cols < 32 ? cols : 32), 256, 0, mmp::stream()>>>(
-      keys, n, share, (unsigned)rows, (unsigned)width, (S)scale, (const S *)part.p, out);
+  mmpd::emb_join_kernel<T, JV><<<dim3(shares < 128 ? shares : 128, cols < 32 ? cols : 32), 256, 0, mmp::stream()>>>(
+      keys, n, share, (unsigned)width, (S)scale, (const S *)part.p, runs, list, out);
   MMP_LAUNCH_CHECK("embedding_grad join");
   return MMP_OK;
 }
@@ -649,16 +678,16 @@ int run_emb_grad(const void *ids_, int64_t n, const void *grad_, int64_t g_strid
   }
   int bits = 1;
   while ((INT64_C(1) << bits) <= rows) ++bits;  // the key `rows` included
-  const FastDiv wd = emb_div((unsigned)width);
   int *err = mmp::device_error_word();
   EmbBuf mem;
   const size_t np = ((size_t)n + 3) & ~(size_t)3;
-  unsigned *keys, *order;
+  unsigned *keys, *order, *runs;
   if (n <= mmpd::kEmbCluster) {
-    int rc = mem.alloc(np * 8);
+    int rc = mem.alloc(np * 8 + 16);
     if (rc) return rc;
     keys = (unsigned *)mem.p;
     order = keys + np;
+    runs = order + np;
     const int items = (int)((n + mmpd::kSortThreads * mmpd::kSortRanks - 1) / (mmpd::kSortThreads * mmpd::kSortRanks));
     const int passes = (bits + 7) / 8, digit = (bits + passes - 1) / passes;
     // one block an SM; clusters of eight fill 16 SMs of each of the GPU's parts
@@ -672,10 +701,11 @@ int run_emb_grad(const void *ids_, int64_t n, const void *grad_, int64_t g_strid
     auto fn = mmpd::emb_sort_kernel<T, I>;
     MMP_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     fn<<<clusters * mmpd::kSortRanks, mmpd::kSortThreads, smem, mmp::stream()>>>(
-        ids, (unsigned)n, rows, padding, items, passes, digit, keys, order, wd, out, (unsigned)(seen * 8), err);
+        ids, (unsigned)n, rows, padding, items, passes, digit, keys, order, (unsigned)width, out, (unsigned)(seen * 8),
+        runs, err);
     MMP_LAUNCH_CHECK("embedding_grad sort");
   } else {
-    int rc = mem.alloc(np * 16);
+    int rc = mem.alloc(np * 16 + 16);
     if (rc) return rc;
     unsigned *const kb[2] = {(unsigned *)mem.p, (unsigned *)mem.p + np};
     unsigned *const ob[2] = {kb[1] + np, kb[1] + 2 * np};
@@ -687,14 +717,15 @@ int run_emb_grad(const void *ids_, int64_t n, const void *grad_, int64_t g_strid
     if (rc) return rc;
     keys = kb[cur];
     order = ob[cur];
+    runs = ob[1] + np;
     const unsigned blocks = (unsigned)mmp::sm_count() * 8;
-    mmpd::emb_gaps_kernel<T><<<blocks, 256, 16384, mmp::stream()>>>(keys, (unsigned)n, rows, wd, out, 131072u, err);
+    mmpd::emb_gaps_kernel<T><<<blocks, 256, 16384, mmp::stream()>>>(keys, (unsigned)n, rows, (unsigned)width, out, 131072u, runs, err);
     MMP_LAUNCH_CHECK("embedding_grad zeros");
   }
-  if (vec == WIDE) return emb_sum<T, I, WIDE>(keys, order, (unsigned)n, grad, g_stride, rows, width, scale, out);
+  if (vec == WIDE) return emb_sum<T, I, WIDE>(keys, order, runs, (unsigned)n, grad, g_stride, rows, width, scale, out);
   if constexpr (sizeof(T) == 2)
-    if (vec == 2) return emb_sum<T, I, 2>(keys, order, (unsigned)n, grad, g_stride, rows, width, scale, out);
-  return emb_sum<T, I, 1>(keys, order, (unsigned)n, grad, g_stride, rows, width, scale, out);
+    if (vec == 2) return emb_sum<T, I, 2>(keys, order, runs, (unsigned)n, grad, g_stride, rows, width, scale, out);
+  return emb_sum<T, I, 1>(keys, order, runs, (unsigned)n, grad, g_stride, rows, width, scale, out);
 }
 
 }  // namespace

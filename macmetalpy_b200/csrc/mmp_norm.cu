@@ -19,7 +19,7 @@
 namespace mmpd {
 
 constexpr int kNormTable = 512;
-constexpr int kNormThreads = 512;
+constexpr int kNormThreads = 256;
 constexpr long long kNormChunk = 16384;  // elements
 
 struct NormEntry {
@@ -61,22 +61,49 @@ __device__ __forceinline__ double norm_block_sum(double v) {
   return v;
 }
 
+template <class T> struct alignas(16) NormVec { T v[16 / sizeof(T)]; };
+
+// The sum of a chunk's squares.  16-byte loads, four ahead, where the chunk is
+// aligned to them (chunks start a multiple of 16 bytes into their array).
 template <class T>
-__device__ __forceinline__ double norm_chunk(const T *x, long long n) {
+__device__ __forceinline__ double norm_chunk(const T *x, int n) {
+  constexpr int PE = 16 / (int)sizeof(T);
   double acc = 0.0;
-  for (long long i = threadIdx.x; i < n; i += kNormThreads) {
-    const double v = (double)Cvt<double, T>::f(x[i]);
-    acc = fma(v, v, acc);
+  int done = 0;
+  if (((uintptr_t)x & 15) == 0) {
+    const NormVec<T> *p = reinterpret_cast<const NormVec<T> *>(x);
+    const int pieces = n / PE;
+    for (int i = threadIdx.x; i < pieces; i += 4 * kNormThreads) {
+      NormVec<T> v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (i + u * kNormThreads < pieces) v[u] = p[i + u * kNormThreads];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (i + u * kNormThreads < pieces) {
+#pragma unroll
+          for (int e = 0; e < PE; ++e) {
+            const double f = Cvt<double, T>::f(v[u].v[e]);
+            acc = fma(f, f, acc);
+          }
+        }
+      }
+    }
+    done = pieces * PE;
+  }
+  for (int i = done + threadIdx.x; i < n; i += kNormThreads) {
+    const double f = Cvt<double, T>::f(x[i]);
+    acc = fma(f, f, acc);
   }
   return acc;
 }
 
-__global__ void __launch_bounds__(kNormThreads) norm_sum_kernel(const __grid_constant__ NormTable t, double *partial) {
+__global__ void __launch_bounds__(kNormThreads, 4) norm_sum_kernel(const __grid_constant__ NormTable t, double *partial) {
   double acc = 0.0;
   for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
     const NormEntry &e = norm_find(t, c);
     const long long at = (long long)(c - e.first) * kNormChunk;
-    const long long n = e.n - at < kNormChunk ? e.n - at : kNormChunk;
+    const int n = (int)(e.n - at < kNormChunk ? e.n - at : kNormChunk);
     if (e.dtype == MMP_DT_FLOAT16) acc += norm_chunk((const __half *)e.x + at, n);
     else if (e.dtype == MMP_DT_FLOAT32) acc += norm_chunk((const float *)e.x + at, n);
     else acc += norm_chunk((const double *)e.x + at, n);
@@ -97,11 +124,33 @@ __device__ __forceinline__ double norm_total(const double *partial, int n) {
 }
 
 template <class T, class S>
-__device__ __forceinline__ void norm_scale(const T *x, T *y, long long n, S coef) {
-  for (long long i = threadIdx.x; i < n; i += kNormThreads) y[i] = Cvt<T, S>::f(Cvt<S, T>::f(x[i]) * coef);
+__device__ __forceinline__ void norm_scale(const T *x, T *y, int n, S coef) {
+  constexpr int PE = 16 / (int)sizeof(T);
+  int done = 0;
+  if ((((uintptr_t)x | (uintptr_t)y) & 15) == 0) {
+    const NormVec<T> *p = reinterpret_cast<const NormVec<T> *>(x);
+    NormVec<T> *q = reinterpret_cast<NormVec<T> *>(y);
+    const int pieces = n / PE;
+    for (int i = threadIdx.x; i < pieces; i += 4 * kNormThreads) {
+      NormVec<T> v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (i + u * kNormThreads < pieces) v[u] = p[i + u * kNormThreads];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (i + u * kNormThreads < pieces) {
+#pragma unroll
+          for (int e = 0; e < PE; ++e) v[u].v[e] = Cvt<T, S>::f(Cvt<S, T>::f(v[u].v[e]) * coef);
+          q[i + u * kNormThreads] = v[u];
+        }
+      }
+    }
+    done = pieces * PE;
+  }
+  for (int i = done + threadIdx.x; i < n; i += kNormThreads) y[i] = Cvt<T, S>::f(Cvt<S, T>::f(x[i]) * coef);
 }
 
-__global__ void __launch_bounds__(kNormThreads) norm_scale_kernel(const __grid_constant__ NormTable t,
+__global__ void __launch_bounds__(kNormThreads, 4) norm_scale_kernel(const __grid_constant__ NormTable t,
                                                                   const double *partial, int npartial, double max_norm,
                                                                   int norm_f64, void *norm_out) {
   const double norm = norm_total(partial, npartial);
@@ -110,11 +159,11 @@ __global__ void __launch_bounds__(kNormThreads) norm_scale_kernel(const __grid_c
     else *(float *)norm_out = (float)norm;
   }
   const double coef = norm <= max_norm ? 1.0 : max_norm / norm;
-  for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
+  for (int c = t.chunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {  // what was read last lies in L2
     const NormEntry &e = norm_find(t, c);
     if (coef == 1.0 && e.x == e.y) continue;  // in place, nothing to scale
     const long long at = (long long)(c - e.first) * kNormChunk;
-    const long long n = e.n - at < kNormChunk ? e.n - at : kNormChunk;
+    const int n = (int)(e.n - at < kNormChunk ? e.n - at : kNormChunk);
     if (e.dtype == MMP_DT_FLOAT16) norm_scale((const __half *)e.x + at, (__half *)e.y + at, n, (float)coef);
     else if (e.dtype == MMP_DT_FLOAT32) norm_scale((const float *)e.x + at, (float *)e.y + at, n, (float)coef);
     else norm_scale((const double *)e.x + at, (double *)e.y + at, n, coef);
@@ -167,7 +216,7 @@ extern "C" int mmp_global_norm(int64_t count, const int *dtypes, const void *con
   }
   cudaStream_t st = mmp::stream();
   if (!st) return mmp::set_error(MMP_E_CUDA, "no CUDA device available");
-  const int64_t most = (int64_t)mmp::sm_count() * 4;
+  const int64_t most = (int64_t)mmp::sm_count() * 8;
   const int64_t launches = count ? (count + mmpd::kNormTable - 1) / mmpd::kNormTable : 1;
   double *partial = nullptr;
   MMP_CUDA_TRY(cudaMallocAsync((void **)&partial, (size_t)(launches * most) * sizeof(double), st));
