@@ -18,14 +18,14 @@ the same bits for equal calls.
 from __future__ import annotations
 
 import bisect
-import ctypes
 import math
+import operator
 
 import numpy as np
 
 from . import _cuda_backend as _cb
 from ._dtypes import MMP_CODES, resolve_dtype
-from .ndarray import ndarray
+from .ndarray import _c_contiguous_strides, ndarray
 
 __all__ = ["linear_recurrence", "linear_recurrence_grad", "embedding", "embedding_grad", "global_norm",
            "clip_by_global_norm"]
@@ -75,7 +75,7 @@ def _span(a: ndarray):
 
 
 def _overlap(a: ndarray, b: ndarray) -> bool:
-    if a.size == 0 or b.size == 0:
+    if a._buffer is not b._buffer or a.size == 0 or b.size == 0:  # a buffer is one allocation
         return False
     a0, a1 = _span(a)
     b0, b1 = _span(b)
@@ -90,14 +90,17 @@ def _same(a: ndarray, b: ndarray) -> bool:
 # ------------------------------------------------------------------ recurrence
 
 def _split(shape, axis):
-    outer = math.prod(shape[:axis]) if axis else 1
-    return outer, shape[axis], math.prod(shape[axis + 1:])
+    if len(shape) == 3 and axis == 1:
+        return shape
+    return math.prod(shape[:axis]), shape[axis], math.prod(shape[axis + 1:])
 
 
 def _strides3(a: ndarray, axis: int):
     """(outer, step) element strides of ``a`` seen as (outer, steps, inner)
     with inner contiguous, or None if no such strides exist."""
     shape, st = a._shape, a._strides
+    if len(shape) == 3 and axis == 1 and (st[2] == 1 or shape[2] == 1):  # (batch, steps, width)
+        return (st[0] if shape[0] != 1 else 0), st[1]
     run = 1
     for n, s in zip(reversed(shape[axis + 1:]), reversed(st[axis + 1:])):
         if n != 1 and s != run:
@@ -132,9 +135,14 @@ def _out3(out, shape, dt, axis, what, name, inputs, same_ok):
     if out is not None:
         _check_out(out, shape, dt, what, name)
         r = _strides3(out, axis)
-        writable = r is not None and all(s != 0 or n <= 1 for n, s in zip(out._shape, out._strides))
-        if writable and not any(_overlap(out, b) and not (ok and _same(out, b)) for b, ok in zip(inputs, same_ok)):
-            return out, r[0], r[1]
+        ok = r is not None and (0 not in out._strides or all(s != 0 or n <= 1
+                                                             for n, s in zip(out._shape, out._strides)))
+        if ok:
+            for b, same in zip(inputs, same_ok):
+                if out._buffer is b._buffer and _overlap(out, b) and not (same and _same(out, b)):
+                    break
+            else:
+                return out, r[0], r[1]
     new = ndarray._empty(shape, dt)
     so, st = _strides3(new, axis)
     return new, so, st
@@ -154,8 +162,10 @@ def _state(s, shape, dt, what, name):
     s = _arr(s, what)
     if s._shape != shape:
         raise ValueError(f"{what}: {name} has shape {s._shape}, needs {shape}")
-    _floating(s._dtype, what)
-    return _cast(s, dt)._ensure_contiguous()
+    if s._dtype != dt:
+        _floating(s._dtype, what)
+        s = s.astype(dt)
+    return s if s._buffer is not None and s._strides == _c_contiguous_strides(shape) else s._ensure_contiguous()
 
 
 def _p(a):
@@ -209,7 +219,10 @@ def linear_recurrence(a, x, h0=None, *, axis=-2, gated=False, out=None, state_ou
     if state_out is not None:
         _check_out(state_out, sshape, sdt, what, "state_out")
         state = state_out
-        if not state._is_c_contiguous() or any(_overlap(state, b) for b in (a, x, h)) or (
+        buf = state._buffer
+        if state._strides != _c_contiguous_strides(sshape) or (
+                (buf is a._buffer or buf is x._buffer or buf is h._buffer)
+                and any(_overlap(state, b) for b in (a, x, h))) or (
                 h0 is not None and _overlap(state, h0) and not _same(state, h0)):
             state = ndarray._empty(sshape, sdt)
     _cb.check(_cb.lib.mmp_recurrence(MMP_CODES[dt], bool(gated), outer, steps, inner, a._ptr, a_so, a_st, x._ptr,
@@ -283,8 +296,8 @@ def linear_recurrence_grad(a, x, h, grad, h0=None, *, axis=-2, gated=False, grad
         gh0 = out[2]
         if gh0 is not None:
             _check_out(gh0, sshape, sdt, what, "out[2]")
-            if not gh0._is_c_contiguous() or any(_overlap(gh0, b) for b in inputs + [ga, gx]
-                                                 if not (b is grad_state and _same(gh0, b))):
+            if not gh0._is_c_contiguous() or any(_overlap(gh0, b) and not (b is grad_state and _same(gh0, b))
+                                                 for b in inputs + [ga, gx]):
                 gh0 = None
         if gh0 is None:
             gh0 = ndarray._empty(sshape, sdt)
@@ -399,38 +412,115 @@ def embedding_grad(ids, grad, num_rows, scale=1.0, *, padding_idx=None, out=None
 
 # ------------------------------------------------------------------ global norm
 
-def _norm_call(arrays, outs, max_norm, norm_out, what):
-    """The norm of ``arrays`` (a list of contiguous arrays), and with ``outs`` the
-    clipped arrays."""
-    n = len(arrays)
-    f64 = False
-    codes, ptrs, sizes = (ctypes.c_int * n)(), (ctypes.c_void_p * n)(), (ctypes.c_int64 * n)()
-    for i, a in enumerate(arrays):
-        dt = a._dtype
-        f64 = f64 or dt == _F64
-        codes[i], ptrs[i], sizes[i] = MMP_CODES[dt], a._ptr, a.size
-    yptrs = None
-    if outs is not None:
-        yptrs = (ctypes.c_void_p * n)(*[o._ptr for o in outs])
-    ndt = _F64 if f64 else _F32
-    norm = norm_out
+_LAYOUT = operator.attrgetter("_buffer", "_offset", "_shape", "_strides", "_dtype")
+_PTR = operator.attrgetter("ptr")
+_FLOATS = {MMP_CODES[np.dtype(t)] for t in (np.float16, np.float32, np.float64)}
+_ITEM = np.zeros(max(MMP_CODES.values()) + 1, np.int64)  # item size by dtype code
+for _dt, _code in MMP_CODES.items():
+    _ITEM[_code] = _dt.itemsize
+
+
+class _Shapes(dict):
+    """shape -> (C-contiguous strides, size)."""
+
+    def __missing__(self, shape):
+        r = (_c_contiguous_strides(shape), math.prod(shape))
+        if len(self) < 4096:
+            self[shape] = r
+        return r
+
+
+_SHAPES = _Shapes()
+
+
+class _Listed:
+    """A list of C-contiguous floating arrays as the library takes it: addresses,
+    sizes and dtype codes.  Gradients come by the hundred, and a few attribute
+    reads an array are what the host may spend on each (some 0.3 us; checks one
+    by one took 2.5); so whatever does not fit at once is left to `of_any`."""
+
+    __slots__ = ("arrays", "shapes", "dtypes", "codes", "ptrs", "sizes", "ends")
+
+    @classmethod
+    def of(cls, arrays):
+        """None if one of the arrays is lazy, strided or not an array of floats."""
+        if not arrays or set(map(type, arrays)) != {ndarray}:
+            return None
+        bufs, offs, shapes, strides, dts = zip(*map(_LAYOUT, arrays))
+        if None in bufs:  # lazy
+            return None
+        want, sizes = zip(*map(_SHAPES.__getitem__, shapes))
+        codes = tuple(map(MMP_CODES.get, dts))
+        if strides != want or not _FLOATS.issuperset(codes):
+            return None
+        r = cls()
+        r.arrays, r.shapes, r.dtypes = arrays, shapes, dts
+        r.codes = np.array(codes, np.int32)
+        item = _ITEM[r.codes]
+        r.sizes = np.array(sizes, np.int64)
+        r.ptrs = np.array(list(map(_PTR, bufs)), np.int64)
+        if any(offs):
+            r.ptrs += np.array(offs, np.int64) * item
+        r.ends = r.ptrs + r.sizes * item
+        return r
+
+    @classmethod
+    def of_any(cls, arrays, what):
+        arrays = [_arr(a, what) for a in arrays]
+        for a in arrays:
+            _floating(a._dtype, what)
+        arrays = [a._ensure_contiguous() for a in arrays]
+        for i, a in enumerate(arrays):
+            if a._strides != _c_contiguous_strides(a._shape):  # axes of one entry: the same memory
+                arrays[i] = a._view(a._shape, _c_contiguous_strides(a._shape), a._offset)
+        r = cls.of(arrays)
+        if r is None:
+            r = cls()
+            r.arrays, r.shapes, r.dtypes = [], (), ()
+            r.codes = np.zeros(0, np.int32)
+            r.ptrs = r.sizes = r.ends = np.zeros(0, np.int64)
+        return r
+
+
+def _apart(lists, norm_out):
+    """Whether no two arrays of the lists, and the norm's, share memory."""
+    starts, ends = [r.ptrs for r in lists], [r.ends for r in lists]
     if norm_out is not None:
-        _check_out(norm_out, (), ndt, what, "out" if outs is None else "norm_out")
-        if any(_overlap(norm_out, b) for b in list(arrays) + list(outs or ())):
-            raise ValueError(f"{what}: the norm's array overlaps one of the arrays")
+        p = norm_out._ptr
+        starts.append(np.array([p], np.int64))
+        ends.append(np.array([p + norm_out._dtype.itemsize], np.int64))
+    starts, ends = np.concatenate(starts), np.concatenate(ends)
+    order = np.argsort(starts)
+    return bool((ends[order[:-1]] <= starts[order[1:]]).all())
+
+
+def _host(a: np.ndarray) -> int:
+    return a.__array_interface__["data"][0]
+
+
+def _norm_call(src, dst, max_norm, norm_out, what, name, apart=False):
+    """The norm of the arrays of `src`, and with `dst` the clipped arrays
+    (`apart`: the norm's array is known to overlap none)."""
+    ndt = _F64 if _F64 in src.dtypes else _F32
+    if norm_out is not None:
+        _check_out(norm_out, (), ndt, what, name)
+        p = norm_out._ptr
+        for r in () if apart else (src, dst) if dst is not None else (src,):
+            if ((r.ptrs < p + ndt.itemsize) & (p < r.ends)).any():
+                raise ValueError(f"{what}: {name} overlaps one of the arrays")
+        norm = norm_out
     else:
         norm = ndarray._empty0(ndt)
-    _cb.check(_cb.lib.mmp_global_norm(n, codes, ptrs, yptrs, sizes, max_norm, MMP_CODES[ndt], norm._ptr), what)
+    _cb.check(_cb.lib.mmp_global_norm(len(src.codes), _host(src.codes), _host(src.ptrs),
+                                      None if dst is None else _host(dst.ptrs), _host(src.sizes), max_norm,
+                                      MMP_CODES[ndt], norm._ptr), what)
     return norm
 
 
 def _norm_list(arrays, what):
-    if isinstance(arrays, ndarray) or not isinstance(arrays, (list, tuple)):
+    if not isinstance(arrays, (list, tuple)):
         raise TypeError(f"{what} takes a list of arrays, got {type(arrays).__name__}")
-    res = [_arr(a, what) for a in arrays]
-    for a in res:
-        _floating(a._dtype, what)
-    return res
+    return _Listed.of(arrays) or _Listed.of_any(arrays, what)
 
 
 def global_norm(arrays, *, out=None):
@@ -441,7 +531,7 @@ def global_norm(arrays, *, out=None):
     arrays is.  An empty list has norm 0.
     """
     what = "global_norm"
-    return _norm_call([a._ensure_contiguous() for a in _norm_list(arrays, what)], None, 0.0, out, what)
+    return _norm_call(_norm_list(arrays, what), None, 0.0, out, what, "out")
 
 
 def clip_by_global_norm(arrays, max_norm, *, out=None, norm_out=None):
@@ -458,23 +548,32 @@ def clip_by_global_norm(arrays, max_norm, *, out=None, norm_out=None):
     scaled.  ``norm_out`` receives the norm.
     """
     what = "clip_by_global_norm"
-    arrays = _norm_list(arrays, what)
+    src = _norm_list(arrays, what)
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"{what}: max_norm must be >= 0, got {max_norm}")
-    srcs = [a._ensure_contiguous() for a in arrays]
     if out is None:
-        outs = res = [ndarray._empty(a._shape, a._dtype) for a in srcs]
+        res = [ndarray._empty(s, d) for s, d in zip(src.shapes, src.dtypes)]
+        dst = _Listed.of(res) or _Listed.of_any(res, what)
+        return res, _norm_call(src, dst, max_norm, norm_out, what, "norm_out")
+    if not isinstance(out, (list, tuple)) or len(out) != len(src.codes):
+        raise ValueError(f"{what}: out must be a list of {len(src.codes)} arrays")
+    res = list(out)
+    # the usual cases: the arrays themselves, or others that are all apart
+    if out is arrays and src.arrays is arrays:
+        if _apart((src,), norm_out if norm_out.__class__ is ndarray else None):
+            return res, _norm_call(src, src, max_norm, norm_out, what, "norm_out", True)
     else:
-        if not isinstance(out, (list, tuple)) or len(out) != len(arrays):
-            raise ValueError(f"{what}: out must be a list of {len(arrays)} arrays")
-        res = list(out)
-        outs = []
-        for o, a in zip(res, srcs):
-            _check_out(o, a._shape, a._dtype, what)
-            outs.append(o)
-        _norm_outs(outs, srcs)
-    norm = _norm_call(srcs, outs, max_norm, norm_out, what)
+        dst = _Listed.of(res)
+        if dst is not None and dst.shapes == src.shapes and dst.dtypes == src.dtypes:
+            same = bool((dst.ptrs == src.ptrs).all())
+            if _apart((src,) if same else (src, dst), norm_out if norm_out.__class__ is ndarray else None):
+                return res, _norm_call(src, dst, max_norm, norm_out, what, "norm_out", True)
+    for o, s, d in zip(res, src.shapes, src.dtypes):
+        _check_out(o, s, d, what)
+    outs = list(res)
+    _norm_outs(outs, src.arrays)
+    norm = _norm_call(src, _Listed.of_any(outs, what), max_norm, norm_out, what, "norm_out")
     for o, r in zip(outs, res):
         if o is not r:
             r[...] = o
