@@ -18,7 +18,7 @@
 
 namespace mmpd {
 
-constexpr int kNormTable = 512;
+constexpr int kNormTable = 512, kNormFew = 32;  // arrays a launch; a short list travels in 1 KB, not 16
 constexpr int kNormThreads = 256;
 constexpr long long kNormChunk = 16384;  // elements
 
@@ -29,13 +29,13 @@ struct NormEntry {
   int first;  // chunks of the entries before this one
   int dtype;
 };
-struct NormTable {
-  NormEntry e[kNormTable];
+template <int N> struct NormTable {
   int count;
   int chunks;
+  NormEntry e[N];
 };
 
-__device__ __forceinline__ const NormEntry &norm_find(const NormTable &t, int chunk) {
+template <int N> __device__ __forceinline__ const NormEntry &norm_find(const NormTable<N> &t, int chunk) {
   int lo = 0, hi = t.count - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
@@ -98,7 +98,9 @@ __device__ __forceinline__ double norm_chunk(const T *x, int n) {
   return acc;
 }
 
-__global__ void __launch_bounds__(kNormThreads, 4) norm_sum_kernel(const __grid_constant__ NormTable t, double *partial) {
+template <int N>
+__global__ void __launch_bounds__(kNormThreads, 4) norm_sum_kernel(const __grid_constant__ NormTable<N> t,
+                                                                   double *partial) {
   double acc = 0.0;
   for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
     const NormEntry &e = norm_find(t, c);
@@ -150,7 +152,8 @@ __device__ __forceinline__ void norm_scale(const T *x, T *y, int n, S coef) {
   for (int i = done + threadIdx.x; i < n; i += kNormThreads) y[i] = Cvt<T, S>::f(Cvt<S, T>::f(x[i]) * coef);
 }
 
-__global__ void __launch_bounds__(kNormThreads, 4) norm_scale_kernel(const __grid_constant__ NormTable t,
+template <int N>
+__global__ void __launch_bounds__(kNormThreads, 4) norm_scale_kernel(const __grid_constant__ NormTable<N> t,
                                                                   const double *partial, int npartial, double max_norm,
                                                                   int norm_f64, void *norm_out) {
   const double norm = norm_total(partial, npartial);
@@ -175,10 +178,21 @@ __global__ void __launch_bounds__(kNormThreads, 4) norm_scale_kernel(const __gri
 namespace {
 
 using mmpd::NormTable;
+using mmpd::kNormFew;
+using mmpd::kNormTable;
+
+// The first entries of a table, for the kernels of short lists.
+NormTable<kNormFew> norm_few(const NormTable<kNormTable> &t) {
+  NormTable<kNormFew> f;
+  f.count = t.count;
+  f.chunks = t.chunks;
+  for (int i = 0; i < t.count; ++i) f.e[i] = t.e[i];
+  return f;
+}
 
 // The next part of the list, from array *at on: at most kNormTable arrays
 // with elements.
-int norm_fill(NormTable &t, int64_t *at, int64_t count, const int *dtypes, const void *const *x, void *const *y,
+int norm_fill(NormTable<kNormTable> &t, int64_t *at, int64_t count, const int *dtypes, const void *const *x, void *const *y,
               const int64_t *sizes) {
   t.count = 0;
   long long chunks = 0;
@@ -220,13 +234,16 @@ extern "C" int mmp_global_norm(int64_t count, const int *dtypes, const void *con
   const int64_t launches = count ? (count + mmpd::kNormTable - 1) / mmpd::kNormTable : 1;
   double *partial = nullptr;
   MMP_CUDA_TRY(cudaMallocAsync((void **)&partial, (size_t)(launches * most) * sizeof(double), st));
-  static thread_local NormTable t;
+  static thread_local NormTable<kNormTable> t;
   int rc = MMP_OK, npartial = 0;
   for (int64_t at = 0; at < count && !rc;) {
     rc = norm_fill(t, &at, count, dtypes, x, y, sizes);
     if (rc || !t.chunks) continue;
     const int grid = (int)(t.chunks < most ? t.chunks : most);
-    mmpd::norm_sum_kernel<<<grid, mmpd::kNormThreads, 0, st>>>(t, partial + npartial);
+    if (t.count <= kNormFew)
+      mmpd::norm_sum_kernel<<<grid, mmpd::kNormThreads, 0, st>>>(norm_few(t), partial + npartial);
+    else
+      mmpd::norm_sum_kernel<<<grid, mmpd::kNormThreads, 0, st>>>(t, partial + npartial);
     npartial += grid;
   }
   // with one table the one just filled serves both kernels
@@ -237,8 +254,12 @@ extern "C" int mmp_global_norm(int64_t count, const int *dtypes, const void *con
     else t.count = t.chunks = 0;
     if (rc) break;
     const int grid = (int)(t.chunks < 1 ? 1 : t.chunks < most ? t.chunks : most);
-    mmpd::norm_scale_kernel<<<grid, mmpd::kNormThreads, 0, st>>>(t, partial, npartial, max_norm,
-                                                                norm_dtype == MMP_FLOAT64, first ? norm : nullptr);
+    void *const to = first ? norm : nullptr;
+    const int f64 = norm_dtype == MMP_FLOAT64;
+    if (t.count <= kNormFew)
+      mmpd::norm_scale_kernel<<<grid, mmpd::kNormThreads, 0, st>>>(norm_few(t), partial, npartial, max_norm, f64, to);
+    else
+      mmpd::norm_scale_kernel<<<grid, mmpd::kNormThreads, 0, st>>>(t, partial, npartial, max_norm, f64, to);
     first = false;
   }
   const cudaError_t le = cudaGetLastError();

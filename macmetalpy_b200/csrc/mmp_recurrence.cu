@@ -625,6 +625,92 @@ __global__ void __launch_bounds__(32 * (kRecWarps + 1), 2) rec_kernel(
   }
 }
 
+// A few steps (a decode step's one, a short segment): a thread has VEC
+// neighbouring chains and walks their steps, B of them loaded at once.
+template <class T, int VEC, bool GRAD, bool GATED>
+__global__ void __launch_bounds__(128) rec_short_kernel(const __grid_constant__ RecArgs g) {
+  typedef typename RecState<T>::type S;
+  typedef RecVec<T, VEC> V;
+  constexpr int SV = VEC * (int)sizeof(S) > 16 ? 16 / (int)sizeof(S) : VEC;  // states move 16 bytes at a time
+  typedef RecVec<S, SV> VS;
+  constexpr int NA = GRAD ? (GATED ? 4 : 3) : 2, NO = GRAD ? 2 : 1, B = 4;
+  const long long grp = blockIdx.x * 128ll + threadIdx.x, per = g.inner / VEC;
+  if (grp >= g.outer * per) return;
+  const long long o = grp / per, i = (grp - o * per) * VEC, chain = o * g.inner + i;
+  const T *in[NA];
+#pragma unroll
+  for (int q = 0; q < NA; ++q) in[q] = (const T *)g.in[q].p + o * g.in[q].so + i;
+  T *out[NO];
+#pragma unroll
+  for (int q = 0; q < NO; ++q) out[q] = (T *)const_cast<void *>(g.out[q].p) + o * g.out[q].so + i;
+  auto states = [&](const void *p, S *to) {
+#pragma unroll
+    for (int v = 0; v < VEC; v += SV) {
+      VS r;
+#pragma unroll
+      for (int e = 0; e < SV; ++e) r.v[e] = S(0);
+      if (p) r = *reinterpret_cast<const VS *>((const S *)p + chain + v);
+#pragma unroll
+      for (int e = 0; e < SV; ++e) to[v + e] = r.v[e];
+    }
+  };
+  S s[VEC];
+  states(g.seed, s);
+  for (int k0 = 0; k0 < g.steps; k0 += B) {
+    V raw[B][NA];
+#pragma unroll
+    for (int j = 0; j < B; ++j) {
+      const long long t = GRAD ? g.steps - 1 - (k0 + j) : k0 + j;
+#pragma unroll
+      for (int q = 0; q < NA; ++q)
+        if (k0 + j < g.steps && (!GRAD || q != 2 || t > 0))
+          raw[j][q] = *reinterpret_cast<const V *>(in[q] + (GRAD && q == 2 ? t - 1 : t) * g.in[q].st);
+    }
+#pragma unroll
+    for (int j = 0; j < B; ++j) {
+      if (k0 + j >= g.steps) break;
+      const long long t = GRAD ? g.steps - 1 - (k0 + j) : k0 + j;
+      S hp[GRAD ? VEC : 1];
+      if constexpr (GRAD) {
+        if (t > 0) {
+#pragma unroll
+          for (int v = 0; v < VEC; ++v) hp[v] = Cvt<S, T>::f(raw[j][2].v[v]);
+        } else {
+          states(g.h0, hp);
+        }
+      }
+      V r0, r1;
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {
+        S f = Cvt<S, T>::f(raw[j][0].v[v]), rest = S(1);
+        const S x = Cvt<S, T>::f(raw[j][1].v[v]);  // grad in the backward pass
+        if (GATED) rec_gate<T>(f, f, rest);
+        if (!GRAD) {
+          s[v] = fma(f, s[v], GATED ? rest * x : x);
+          r0.v[v] = Cvt<T, S>::f(s[v]);
+        } else {
+          const S gt = x + s[v];
+          r0.v[v] = Cvt<T, S>::f(GATED ? gt * (hp[GRAD ? v : 0] - Cvt<S, T>::f(raw[j][NA - 1].v[v])) * (f * rest)
+                                       : gt * hp[GRAD ? v : 0]);
+          r1.v[v] = Cvt<T, S>::f(GATED ? gt * rest : gt);
+          s[v] = f * gt;
+        }
+      }
+      *reinterpret_cast<V *>(out[0] + t * g.out[0].st) = r0;
+      if (GRAD) *reinterpret_cast<V *>(out[NO - 1] + t * g.out[NO - 1].st) = r1;
+    }
+  }
+  if (g.last) {
+#pragma unroll
+    for (int v = 0; v < VEC; v += SV) {
+      VS r;
+#pragma unroll
+      for (int e = 0; e < SV; ++e) r.v[e] = s[v + e];
+      *reinterpret_cast<VS *>((S *)g.last + chain + v) = r;
+    }
+  }
+}
+
 }  // namespace mmpd
 
 namespace {
@@ -769,10 +855,28 @@ bool rec_tensors(const RecArgs &g, int nin, int chains, long long e) {
   return true;
 }
 
+template <class T, int VEC, bool GRAD, bool GATED>
+int rec_short(const RecArgs &g) {
+  const long long blocks = (g.outer * (g.inner / VEC) + 127) / 128;
+  if (blocks > INT32_MAX) return mmp::set_error(MMP_E_ARG, "recurrence: too many chains");
+  mmpd::rec_short_kernel<T, VEC, GRAD, GATED><<<(unsigned)blocks, 128, 0, mmp::stream()>>>(g);
+  MMP_LAUNCH_CHECK("recurrence");
+  return MMP_OK;
+}
+
 template <bool GRAD, bool GATED>
 int rec_dispatch(int dtype, const RecArgs &g) {
   using namespace mmpd;
   constexpr int nin = GRAD ? (GATED ? 4 : 3) : 2, nout = GRAD ? 2 : 1;
+  // Up to 16 steps (one warp's span) the chains alone are worked on side by
+  // side: 32 x 1 x 2048 float16 takes 7.0 us by the spans' kernel, 3.7 here.
+  if (g.steps <= 16) {
+    const bool states = ((uintptr_t)g.h0 | (uintptr_t)g.seed | (uintptr_t)g.last) % 16 == 0;
+    const bool wide = states && rec_aligned(g, nin, nout, 16, mmp_dtype_size(dtype));
+    if (dtype == MMP_FLOAT16) return wide ? rec_short<__half, 8, GRAD, GATED>(g) : rec_short<__half, 1, GRAD, GATED>(g);
+    if (dtype == MMP_FLOAT32) return wide ? rec_short<float, 4, GRAD, GATED>(g) : rec_short<float, 1, GRAD, GATED>(g);
+    return wide ? rec_short<double, 2, GRAD, GATED>(g) : rec_short<double, 1, GRAD, GATED>(g);
+  }
   if (dtype == MMP_FLOAT16) {
     if (!rec_aligned(g, nin, nout, 4, 2)) return rec_run<__half, 1, kPlain, GRAD, GATED>(g);
     return rec_tensors(g, nin, 64, 2) ? rec_run<__half, 2, kTma, GRAD, GATED>(g)
