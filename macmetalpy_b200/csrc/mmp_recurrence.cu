@@ -868,9 +868,11 @@ template <bool GRAD, bool GATED>
 int rec_dispatch(int dtype, const RecArgs &g) {
   using namespace mmpd;
   constexpr int nin = GRAD ? (GATED ? 4 : 3) : 2, nout = GRAD ? 2 : 1;
-  // Up to 16 steps (one warp's span) the chains alone are worked on side by
-  // side: 32 x 1 x 2048 float16 takes 7.0 us by the spans' kernel, 3.7 here.
-  if (g.steps <= 16) {
+  // Up to 32 steps (backward 16) the chains alone are worked on side by side:
+  // 32 x 1 x 2048 float16 takes 7.0 us by the spans' kernel, 3.7 here; whole
+  // calls at 8 x 24 x 1024 12.0 and 9.0, 64 x 32 x 4096 23.4 and 19.1, but 16 x
+  // 64 x 4096 12.8 and 19.2, backward 8 x 32 x 1024 13.5 and 17.4.
+  if (g.steps <= (GRAD ? 16 : 32)) {
     const bool states = ((uintptr_t)g.h0 | (uintptr_t)g.seed | (uintptr_t)g.last) % 16 == 0;
     const bool wide = states && rec_aligned(g, nin, nout, 16, mmp_dtype_size(dtype));
     if (dtype == MMP_FLOAT16) return wide ? rec_short<__half, 8, GRAD, GATED>(g) : rec_short<__half, 1, GRAD, GATED>(g);
