@@ -180,21 +180,24 @@ struct RecArgs {
 
 constexpr int kRecWarps = 7;  // and one that joins them: 8 warps of 128 registers, two blocks an SM
 
-// Steps of one warp's span, by the bytes that a lane moves a step: 32 KB of
-// ring a stage and block of 8 warps, so that two blocks of three stages fit an
-// SM.
-template <int BYTES, bool GRAD> struct RecSpan { static constexpr int value = (GRAD ? 8 : 16) / (BYTES == 8 ? 2 : 1); };
-
-template <class S> struct alignas(2 * sizeof(S)) RecMap {
-  S a, h;
-};
-
 // How a span's rows reach the ring.  kTma: one tensor copy an array, by one
 // lane of the warp.  kLane: cp.async of each lane's own 4 or 8 bytes (any
 // strides; issuing these takes a third of the warps' time, and their lines on
 // the way are held in what the ring leaves of L1).  kPlain: loads of 2 bytes,
 // for float16 in rows of odd width.
 enum { kPlain, kLane, kTma };
+
+// Steps of one warp's span, by the bytes that a lane moves a step: 28 KB of
+// ring a stage and block of 7 warps, so that two blocks of three stages fit
+// an SM; kLane has half of that, which leaves its lines more of L1 (1 x 65521 x
+// 1001 float32 191 us, 226 with whole stages).
+template <int BYTES, int COPY, bool GRAD> struct RecSpan {
+  static constexpr int value = (GRAD ? 8 : 16) / (BYTES == 8 ? 2 : 1) / (COPY == kLane ? 2 : 1);
+};
+
+template <class S> struct alignas(2 * sizeof(S)) RecMap {
+  S a, h;
+};
 
 template <int COPY> struct RecMaps {};
 struct alignas(64) RecMap3 {
@@ -218,7 +221,7 @@ __global__ void __launch_bounds__(32 * (kRecWarps + 1), 2) rec_kernel(
     const __grid_constant__ RecArgs g, const __grid_constant__ RecMaps<COPY> maps) {
   typedef typename RecState<T>::type S;
   typedef RecVec<T, VEC> V;
-  constexpr int N = RecSpan<(int)sizeof(V), GRAD>::value;
+  constexpr int N = RecSpan<(int)sizeof(V), COPY, GRAD>::value;
   constexpr int NA = GRAD ? (GATED ? 4 : 3) : 2;
   constexpr int NO = GRAD ? 2 : 1;
   constexpr int NC = 32 * VEC;            // chains of the block
@@ -271,13 +274,12 @@ __global__ void __launch_bounds__(32 * (kRecWarps + 1), 2) rec_kernel(
   V *const ring = reinterpret_cast<V *>(s_ring + skew) + (size_t)w * g.stages * (NA * N * 32) + lane;
   const int span = ranks * warps * N;  // steps of the cluster
   const int mine = (rank * warps + w) * N;
-  S carry[VEC];  // the state before the present span of the cluster (joining warp; a block of one warp)
-#pragma unroll
-  for (int v = 0; v < VEC; ++v) carry[v] = active && g.seed ? ((const S *)g.seed)[chain + v] : S(0);
-
   if (w == warps) {
     // The joining warp, beside the warps that compose and replay: a lane has
     // the chains of its group.
+    S carry[VEC];  // the state before the cluster's present span
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) carry[v] = active && g.seed ? ((const S *)g.seed)[chain + v] : S(0);
     if (CLUSTER) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     bool heard = true;
     for (int it = 0; it < g.iters; ++it) {
@@ -408,7 +410,7 @@ __global__ void __launch_bounds__(32 * (kRecWarps + 1), 2) rec_kernel(
   };
   // stages that are filled ahead: all but the one in work and, with a lag,
   // the one that is replayed (unless every span has its own)
-  const int ahead = COPY == kPlain ? 0 : g.stages - (LAG && warps > 1 && g.stages < g.iters ? 2 : 1);
+  const int ahead = COPY == kPlain ? 0 : g.stages - (LAG && g.stages < g.iters ? 2 : 1);
   bool heard = true;
   if constexpr (COPY == kTma) {
     if (lane == 0) {
@@ -563,7 +565,7 @@ __global__ void __launch_bounds__(32 * (kRecWarps + 1), 2) rec_kernel(
   // stages in turn: of the span filled next, composed next, replayed next
   int fill = ahead % g.stages, next = 0, last = 0;
   unsigned phase = 0;
-  for (int it = 0; it < g.iters + (warps > 1 ? LAG : 0); ++it) {
+  for (int it = 0; it < g.iters + LAG; ++it) {
     if (it < g.iters) {
       if constexpr (COPY == kTma) {
         __syncwarp();  // every lane is done with the stage that is filled next
@@ -591,37 +593,23 @@ __global__ void __launch_bounds__(32 * (kRecWarps + 1), 2) rec_kernel(
         phase ^= 1;
       }
     }
-    if (warps == 1) {
+    if (it < g.iters) {
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        s[v] = carry[v];
-        carry[v] = rec_apply(A[v], H[v], carry[v]);
-      }
-      replay(it, last);
+      for (int v = 0; v < VEC; ++v) s_map[it & 1][w][lane * VEC + v] = RecMap<S>{A[v], H[v]};
+      rec_bar_arrive(1 + (it & 1), 32 * (warps + 1));
+    }
+    if (it >= LAG) {
+      const int par = (it - LAG) & 1;
+      rec_bar_sync(3 + par, 32 * (warps + 1));
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) s[v] = s_start[par][w][lane * VEC + v];
+      replay(it - LAG, last);
       if (++last == g.stages) last = 0;
-    } else {
-      if (it < g.iters) {
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) s_map[it & 1][w][lane * VEC + v] = RecMap<S>{A[v], H[v]};
-        rec_bar_arrive(1 + (it & 1), 32 * (warps + 1));
-      }
-      if (it >= LAG) {
-        const int par = (it - LAG) & 1;
-        rec_bar_sync(3 + par, 32 * (warps + 1));
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) s[v] = s_start[par][w][lane * VEC + v];
-        replay(it - LAG, last);
-        if (++last == g.stages) last = 0;
-      }
     }
   }
   if (CLUSTER) {  // no block ends while it may still be sent to
     asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-  }
-  if (g.steps == 0 && g.last && active && w == 0) {
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) ((S *)g.last)[chain + v] = carry[v];
   }
 }
 
@@ -736,7 +724,7 @@ int rec_launch(const RecArgs &g, const mmpd::RecMaps<COPY> &maps, unsigned block
     MMP_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(blocks * ranks);
-  cfg.blockDim = dim3(32, g.warps + (g.warps > 1));  // and the joining warp
+  cfg.blockDim = dim3(32, g.warps + 1);  // and the joining warp
   cfg.dynamicSmemBytes = smem;
   cfg.stream = mmp::stream();
   cudaLaunchAttribute at[1];
@@ -788,7 +776,11 @@ int rec_map_of(mmpd::RecMap3 *map, const RecView &v, const RecArgs &g, int e, in
   const cuuint64_t strides[2] = {(cuuint64_t)s.s1, (cuuint64_t)s.s2};
   const cuuint32_t box[3] = {(cuuint32_t)chains, (cuuint32_t)(swap ? 1 : steps), (cuuint32_t)(swap ? steps : 1)};
   const cuuint32_t one[3] = {1, 1, 1};
-  const CUresult r = enc(&map->m, e == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3,
+  const CUresult r = enc(&map->m,
+                         e == 2   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                         : e == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                  : CU_TENSOR_MAP_DATA_TYPE_FLOAT64,
+                         3,
                          const_cast<void *>(v.p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                          CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -798,7 +790,7 @@ int rec_map_of(mmpd::RecMap3 *map, const RecView &v, const RecArgs &g, int e, in
 
 template <class T, int VEC, int COPY, bool GRAD, bool GATED>
 int rec_run(RecArgs g) {
-  constexpr int N = mmpd::RecSpan<(int)sizeof(T) * VEC, GRAD>::value;
+  constexpr int N = mmpd::RecSpan<(int)sizeof(T) * VEC, COPY, GRAD>::value;
   constexpr int NA = GRAD ? (GATED ? 4 : 3) : 2;
   constexpr int NC = 32 * VEC;
   g.err = mmp::device_error_word();
@@ -812,14 +804,14 @@ int rec_run(RecArgs g) {
   // us in blocks alone and 59 in clusters of two, which run in two waves;
   // 1 x 65521 x 1000 float32 (32 blocks) 606 alone and 186 in clusters of eight
   const long long spans = ((long long)g.steps + N - 1) / N;
-  int warps = 1, ranks = 1;
-  if (spans > 1) warps = spans < mmpd::kRecWarps ? (int)spans : mmpd::kRecWarps;
+  const int warps = spans < mmpd::kRecWarps ? (int)spans : mmpd::kRecWarps;
+  int ranks = 1;
   while (ranks < 8 && blocks * ranks * 2 <= 2 * mmp::sm_count() && (long long)ranks * warps < spans) ranks *= 2;
   if (blocks * ranks > INT32_MAX) return mmp::set_error(MMP_E_ARG, "recurrence: too many chains");
   g.iters = (int)((spans + (long long)warps * ranks - 1) / ((long long)warps * ranks));
   g.warps = warps;
-  const int most = COPY != mmpd::kPlain ? 3 : warps > 1 ? 2 : 1;
-  g.stages = g.iters < most ? (g.iters > 0 ? g.iters : 1) : most;
+  const int most = COPY != mmpd::kPlain ? 3 : 2;
+  g.stages = g.iters < most ? g.iters : most;
   const size_t smem = 128 + (size_t)g.stages * NA * N * warps * 32 * sizeof(T) * VEC;
   mmpd::RecMaps<COPY> maps;
   if constexpr (COPY == mmpd::kTma) {
@@ -847,7 +839,7 @@ bool rec_aligned(const RecArgs &g, int nin, int nout, size_t bytes, size_t e) {
 // Whether tensor copies can take the inputs, and their tiles of `chains` along
 // inner are at least three quarters full.
 bool rec_tensors(const RecArgs &g, int nin, int chains, long long e) {
-  if (g.steps == 0 || g.inner * 4 < (g.inner + chains - 1) / chains * chains * 3) return false;
+  if (g.inner * 4 < (g.inner + chains - 1) / chains * chains * 3) return false;
   if (g.inner > INT32_MAX || g.outer > INT32_MAX) return false;
   RecStrides s;
   for (int i = 0; i < nin; ++i)
@@ -887,7 +879,8 @@ int rec_dispatch(int dtype, const RecArgs &g) {
   if (dtype == MMP_FLOAT32)
     return rec_tensors(g, nin, 32, 4) ? rec_run<float, 1, kTma, GRAD, GATED>(g)
                                       : rec_run<float, 1, kLane, GRAD, GATED>(g);
-  return rec_run<double, 1, kLane, GRAD, GATED>(g);
+  return rec_tensors(g, nin, 32, 8) ? rec_run<double, 1, kTma, GRAD, GATED>(g)
+                                    : rec_run<double, 1, kLane, GRAD, GATED>(g);
 }
 
 }  // namespace

@@ -228,13 +228,15 @@ def test_recurrence_axes_and_views(cp, dt, axis):
     got = cp.linear_recurrence(A[..., :10], A[..., 11:21], axis=axis).get()
     close(three(got), hs, es * UNIT[dt], dt)
     same = cp.linear_recurrence(cp.array(a), cp.array(x), axis=axis).get()
-    np.testing.assert_array_equal(got, same)
+    close(three(same), hs, es * UNIT[dt], dt)
+    ra, rx = a[:, ::-1], x[:, ::-1]
+    hs, es, _, _ = recurrence(three(ra), three(rx), None, False)
     rev = cp.linear_recurrence(A[:, ::-1, :, :10], A[:, ::-1, :, 11:21], axis=axis).get()
-    np.testing.assert_array_equal(rev, cp.linear_recurrence(cp.array(a[:, ::-1].copy()), cp.array(x[:, ::-1].copy()),
-                                                            axis=axis).get())
+    close(three(rev), hs, es * UNIT[dt], dt)
+    oa = np.broadcast_to(base[:1, :1, :1, :10], (4, 37, 6, 10))
+    hs, es, _, _ = recurrence(three(oa), three(x), None, False)
     one = cp.array(base[:1, :1, :1, :10]).broadcast_to((4, 37, 6, 10))
-    np.testing.assert_array_equal(cp.linear_recurrence(one, A[..., 11:21], axis=axis).get(),
-                                  cp.linear_recurrence(one.copy(), cp.array(x), axis=axis).get())
+    close(three(cp.linear_recurrence(one, A[..., 11:21], axis=axis).get()), hs, es * UNIT[dt], dt)
 
 
 @pytest.mark.parametrize("dt", ["float16", "float32"])
@@ -281,10 +283,13 @@ def test_recurrence_unaligned_views(cp, dt, off):
 
 @pytest.mark.parametrize("dt", ["float16", "float32"])
 def test_recurrence_outputs_in_place(cp, dt):
-    """out= over the inputs, into a strided view, over a shifted view of an
-    input; rows of the larger array outside the view stay as they were."""
+    """out= over the inputs gives the same bits; into a strided view, or over a
+    shifted view of an input (rows that start elsewhere may be copied in other
+    spans): within the bound; rows of the larger array outside the view stay
+    as they were."""
     shape = (2, 150, 70)
     a, x, h0, g, gs = rec_inputs(shape, dt, True, 9)
+    hs, es, _, _ = recurrence(a, x, h0, True)
     want = cp.linear_recurrence(cp.array(a), cp.array(x), cp.array(h0), gated=True).get()
     for over in (0, 1):
         A, X = cp.array(a), cp.array(x)
@@ -293,14 +298,14 @@ def test_recurrence_outputs_in_place(cp, dt):
         np.testing.assert_array_equal(r.get(), want)
     big = cp.full((2, 152, 80), 7, dtype=dt)
     r = cp.linear_recurrence(cp.array(a), cp.array(x), cp.array(h0), gated=True, out=big[:, 1:151, 5:75])
-    np.testing.assert_array_equal(r.get(), want)
+    close(r.get(), hs, es * UNIT[dt], dt)
     host = np.full((2, 152, 80), 7, dt)
-    host[:, 1:151, 5:75] = want
+    host[:, 1:151, 5:75] = r.get()
     np.testing.assert_array_equal(big.get(), host)
     X = cp.zeros((2, 151, 70), dtype=dt)
     X[:, :150] = cp.array(x)
     r = cp.linear_recurrence(cp.array(a), X[:, :150], cp.array(h0), gated=True, out=X[:, 1:])
-    np.testing.assert_array_equal(r.get(), want)
+    close(r.get(), hs, es * UNIT[dt], dt)
     dg = [v.get() for v in cp.linear_recurrence_grad(cp.array(a), cp.array(x), cp.array(want), cp.array(g),
                                                      cp.array(h0), gated=True, grad_state=cp.array(gs))]
     A, X, H, G, S = cp.array(a), cp.array(x), cp.array(want), cp.array(g), cp.array(gs)
