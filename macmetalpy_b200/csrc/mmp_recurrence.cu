@@ -799,14 +799,20 @@ int rec_run(RecArgs g) {
   for (const RecView &v : g.out) g.near &= v.st * (long long)sizeof(T) == (int)(v.st * (long long)sizeof(T));
   g.tiles = (g.inner + NC - 1) / NC;
   const long long blocks = COPY == mmpd::kTma ? g.outer * g.tiles : (g.outer * (g.inner / VEC) + 31) / 32;
-  // as many warps a block and blocks a cluster as there are spans for, while
-  // all blocks fit at two an SM: 8 x 2048 x 2048 float16 (256 blocks) takes 46
-  // us in blocks alone and 59 in clusters of two, which run in two waves;
-  // 1 x 65521 x 1000 float32 (32 blocks) 606 alone and 186 in clusters of eight
+  // As many warps a block as there are spans for, and blocks a cluster while
+  // all fit at two an SM: 1 x 65521 x 1000 float32 (32 blocks) takes 590 us in
+  // blocks alone and 123 in clusters of eight.  Where the blocks are up to one
+  // and a half times the SMs, clusters of four, in more than one wave, even out
+  // what one wave leaves idle (whole calls: 96 blocks float16 gated 114 us in
+  // twos and 93 in fours, its gradient 165 and 136; 160 blocks float32 99 alone
+  // and 94, 192 blocks' gradient 192 and 172; but 128 blocks 113 and 116).  From
+  // there on blocks alone: 256 of 8 x 2048 x 2048 float16 46 us, in fours 71.
   const long long spans = ((long long)g.steps + N - 1) / N;
-  const int warps = spans < mmpd::kRecWarps ? (int)spans : mmpd::kRecWarps;
+  const int warps = spans < mmpd::kRecWarps ? (int)spans : mmpd::kRecWarps, sms = mmp::sm_count();
   int ranks = 1;
-  while (ranks < 8 && blocks * ranks * 2 <= 2 * mmp::sm_count() && (long long)ranks * warps < spans) ranks *= 2;
+  while (ranks < 8 && blocks * ranks * 2 <= 2 * sms && (long long)ranks * warps < spans) ranks *= 2;
+  if (ranks < 4 && blocks * 2 <= 3 * sms && spans >= 8 * warps)  // two rounds of spans at least
+    ranks = spans >= 192 * warps ? 8 : 4;
   if (blocks * ranks > INT32_MAX) return mmp::set_error(MMP_E_ARG, "recurrence: too many chains");
   g.iters = (int)((spans + (long long)warps * ranks - 1) / ((long long)warps * ranks));
   g.warps = warps;
