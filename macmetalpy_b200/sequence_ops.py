@@ -17,7 +17,9 @@ the same bits for equal calls.
 
 from __future__ import annotations
 
+import array
 import bisect
+import itertools
 import math
 import operator
 
@@ -414,10 +416,7 @@ def embedding_grad(ids, grad, num_rows, scale=1.0, *, padding_idx=None, out=None
 
 _LAYOUT = operator.attrgetter("_buffer", "_offset", "_shape", "_strides", "_dtype")
 _PTR = operator.attrgetter("ptr")
-_FLOATS = {MMP_CODES[np.dtype(t)] for t in (np.float16, np.float32, np.float64)}
-_ITEM = np.zeros(max(MMP_CODES.values()) + 1, np.int64)  # item size by dtype code
-for _dt, _code in MMP_CODES.items():
-    _ITEM[_code] = _dt.itemsize
+_KIND = {np.dtype(t): (MMP_CODES[np.dtype(t)], np.dtype(t).itemsize) for t in (np.float16, np.float32, np.float64)}
 
 
 class _Shapes(dict):
@@ -439,7 +438,7 @@ class _Listed:
     reads an array are what the host may spend on each (some 0.3 us; checks one
     by one took 2.5); so whatever does not fit at once is left to `of_any`."""
 
-    __slots__ = ("arrays", "shapes", "dtypes", "codes", "ptrs", "sizes", "ends")
+    __slots__ = ("arrays", "shapes", "dtypes", "codes", "sizes", "ptrs", "ends")
 
     @classmethod
     def of(cls, arrays):
@@ -447,21 +446,20 @@ class _Listed:
         if not arrays or set(map(type, arrays)) != {ndarray}:
             return None
         bufs, offs, shapes, strides, dts = zip(*map(_LAYOUT, arrays))
-        if None in bufs:  # lazy
+        kinds = list(map(_KIND.get, dts))
+        if None in bufs or None in kinds:  # lazy, not floating
             return None
         want, sizes = zip(*map(_SHAPES.__getitem__, shapes))
-        codes = tuple(map(MMP_CODES.get, dts))
-        if strides != want or not _FLOATS.issuperset(codes):
+        if strides != want:
             return None
+        codes, items = zip(*kinds)
         r = cls()
         r.arrays, r.shapes, r.dtypes = arrays, shapes, dts
-        r.codes = np.array(codes, np.int32)
-        item = _ITEM[r.codes]
-        r.sizes = np.array(sizes, np.int64)
-        r.ptrs = np.array(list(map(_PTR, bufs)), np.int64)
+        r.codes, r.sizes = array.array("i", codes), array.array("q", sizes)
+        r.ptrs = list(map(_PTR, bufs))
         if any(offs):
-            r.ptrs += np.array(offs, np.int64) * item
-        r.ends = r.ptrs + r.sizes * item
+            r.ptrs = list(map(operator.add, r.ptrs, map(operator.mul, offs, items)))
+        r.ends = list(map(operator.add, r.ptrs, map(operator.mul, sizes, items)))
         return r
 
     @classmethod
@@ -476,26 +474,25 @@ class _Listed:
         r = cls.of(arrays)
         if r is None:
             r = cls()
-            r.arrays, r.shapes, r.dtypes = [], (), ()
-            r.codes = np.zeros(0, np.int32)
-            r.ptrs = r.sizes = r.ends = np.zeros(0, np.int64)
+            r.arrays, r.shapes, r.dtypes, r.ptrs, r.ends = [], (), (), [], []
+            r.codes, r.sizes = array.array("i"), array.array("q")
         return r
 
 
 def _apart(lists, norm_out):
-    """Whether no two arrays of the lists, and the norm's, share memory."""
-    starts, ends = [r.ptrs for r in lists], [r.ends for r in lists]
+    """Whether no two arrays of the lists, and the norm's, share memory: then, and
+    only then, the sorted ends each lie before the next of the sorted starts."""
+    starts, ends = [], []
+    for r in lists:
+        starts += r.ptrs
+        ends += r.ends
     if norm_out is not None:
         p = norm_out._ptr
-        starts.append(np.array([p], np.int64))
-        ends.append(np.array([p + norm_out._dtype.itemsize], np.int64))
-    starts, ends = np.concatenate(starts), np.concatenate(ends)
-    order = np.argsort(starts)
-    return bool((ends[order[:-1]] <= starts[order[1:]]).all())
-
-
-def _host(a: np.ndarray) -> int:
-    return a.__array_interface__["data"][0]
+        starts.append(p)
+        ends.append(p + norm_out._dtype.itemsize)
+    starts.sort()
+    ends.sort()
+    return all(map(operator.le, ends, itertools.islice(starts, 1, None)))
 
 
 def _norm_call(src, dst, max_norm, norm_out, what, name, apart=False):
@@ -506,13 +503,15 @@ def _norm_call(src, dst, max_norm, norm_out, what, name, apart=False):
         _check_out(norm_out, (), ndt, what, name)
         p = norm_out._ptr
         for r in () if apart else (src, dst) if dst is not None else (src,):
-            if ((r.ptrs < p + ndt.itemsize) & (p < r.ends)).any():
+            if any(a < p + ndt.itemsize and p < b for a, b in zip(r.ptrs, r.ends)):
                 raise ValueError(f"{what}: {name} overlaps one of the arrays")
         norm = norm_out
     else:
         norm = ndarray._empty0(ndt)
-    _cb.check(_cb.lib.mmp_global_norm(len(src.codes), _host(src.codes), _host(src.ptrs),
-                                      None if dst is None else _host(dst.ptrs), _host(src.sizes), max_norm,
+    x = array.array("q", src.ptrs)
+    y = None if dst is None else array.array("q", dst.ptrs)
+    _cb.check(_cb.lib.mmp_global_norm(len(src.codes), src.codes.buffer_info()[0], x.buffer_info()[0],
+                                      None if y is None else y.buffer_info()[0], src.sizes.buffer_info()[0], max_norm,
                                       MMP_CODES[ndt], norm._ptr), what)
     return norm
 
@@ -566,7 +565,7 @@ def clip_by_global_norm(arrays, max_norm, *, out=None, norm_out=None):
     else:
         dst = _Listed.of(res)
         if dst is not None and dst.shapes == src.shapes and dst.dtypes == src.dtypes:
-            same = bool((dst.ptrs == src.ptrs).all())
+            same = dst.ptrs == src.ptrs
             if _apart((src,) if same else (src, dst), norm_out if norm_out.__class__ is ndarray else None):
                 return res, _norm_call(src, dst, max_norm, norm_out, what, "norm_out", True)
     for o, s, d in zip(res, src.shapes, src.dtypes):
