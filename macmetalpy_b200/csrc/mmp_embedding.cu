@@ -24,6 +24,8 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <type_traits>
+
 #include "mmp_device.cuh"
 #include "mmp_internal.h"
 
@@ -299,13 +301,19 @@ __global__ void __cluster_dims__(kSortRanks, 1, 1) __launch_bounds__(kSortThread
   for (long long i = rank * kSortThreads + tid; i < (rows + 31) / 32; i += kSortRanks * kSortThreads) seen[i] = 0;
   const unsigned place = w * items * 32 + lane;  // this thread's keys: place + 32 e
   const unsigned lt = emb_lanemask_lt();
-  for (int e = 0; e < items; ++e) {
+  long long id[kSortItems];
+#pragma unroll
+  for (int e = 0; e < kSortItems; ++e) {
+    const unsigned i = rank * tile + place + e * 32;
+    id[e] = e < items && i < n ? (long long)ids[i] : padding;
+  }
+#pragma unroll
+  for (int e = 0; e < kSortItems; ++e) {
     const unsigned p = place + e * 32, i = rank * tile + p;
-    const long long id = i < n ? (long long)ids[i] : padding;
-    const bool ok = id >= 0 && id < rows;
-    if (i < n) {
+    if (e < items && i < n) {
+      const bool ok = id[e] >= 0 && id[e] < rows;
       if (!ok) atomicExch(err, 5);
-      buf[0][p] = (unsigned long long)(ok && id != padding ? id : rows) << 32 | i;
+      buf[0][p] = (unsigned long long)(ok && id[e] != padding ? id[e] : rows) << 32 | i;
     }
   }
   for (int pass = 0; pass < passes; ++pass) {
@@ -498,28 +506,62 @@ __global__ void __launch_bounds__(256) emb_sum_kernel(const unsigned *__restrict
       *reinterpret_cast<V *>(out + (size_t)cur * width + c) = r;
     }
   };
-  constexpr int B = 8;
-  for (; i < stop; i += B) {
-    V v[B];
-    unsigned key[B];
+  auto turn = [&](unsigned key) {  // the next token's id
+    if (key != cur) {
+      flush(false);
+      head = false;
+      cur = key;
 #pragma unroll
-    for (int j = 0; j < B; ++j) {
-      key[j] = i + j < stop ? keys[i + j] : rows;
-      if (i + j >= i1 && key[j] != after) key[j] = rows;  // the next share's own
-      if (key[j] < rows) v[j] = *reinterpret_cast<const V *>(grad + (long long)order[i + j] * g_stride + c);
+      for (int e = 0; e < VEC; ++e) acc[e] = S(0);
     }
+  };
+  auto add = [&](const V &v) {
 #pragma unroll
-    for (int j = 0; j < B; ++j) {
-      if (key[j] >= rows) continue;  // past the end, or sorted behind every row
-      if (key[j] != cur) {
-        flush(false);
-        head = false;
-        cur = key[j];
+    for (int e = 0; e < VEC; ++e) acc[e] += Cvt<S, T>::f(v.v[e]);
+  };
+  // B tokens at a time from a multiple of B on (keys and order have that many
+  // entries; what lies outside [i, stop) is passed over): eight, or four where
+  // eight would take more registers than four blocks an SM have
+  constexpr int B = VEC >= 8 ? 4 : 8;
+  for (unsigned b = i / B * B; b < stop; b += B) {
+    unsigned key[B], at[B];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) acc[e] = S(0);
+    for (int j = 0; j < B; j += 4) {
+      *reinterpret_cast<uint4 *>(key + j) = *reinterpret_cast<const uint4 *>(keys + b + j);
+      *reinterpret_cast<uint4 *>(at + j) = *reinterpret_cast<const uint4 *>(order + b + j);
+    }
+    V v[B];
+    if (b >= i && b + B <= i1 && key[B - 1] < rows) {
+#pragma unroll
+      for (int j = 0; j < B; ++j) v[j] = *reinterpret_cast<const V *>(grad + (long long)at[j] * g_stride + c);
+      if (key[0] == cur && key[B - 1] == cur) {
+#pragma unroll
+        for (int j = 0; j < B; ++j) add(v[j]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < B; ++j) {
+          turn(key[j]);
+          add(v[j]);
+        }
+      }
+    } else {
+      unsigned use = 0;
+#pragma unroll
+      for (int j = 0; j < B; ++j) {
+        const unsigned q = b + j;
+        // behind this share only the run that goes on from it
+        if (q >= i && q < stop && key[j] < rows && (q < i1 || key[j] == after)) {
+          use |= 1u << j;
+          v[j] = *reinterpret_cast<const V *>(grad + (long long)at[j] * g_stride + c);
+        }
       }
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) acc[e] += Cvt<S, T>::f(v[j].v[e]);
+      for (int j = 0; j < B; ++j) {
+        if (use >> j & 1) {
+          turn(key[j]);
+          add(v[j]);
+        }
+      }
     }
   }
   flush(far);
@@ -604,15 +646,25 @@ int emb_check(const char *what, int dtype, int ids_dtype, int64_t rows, int64_t 
   return MMP_OK;
 }
 
-// Elements that every row can be moved in at once: 16 bytes where width,
-// strides and pointers allow it, 4 bytes for float16 in rows of even width,
-// else one.
+// Elements that every row can be moved in at once: 16, 8 or 4 bytes where
+// width, strides and pointers allow it, else one.
 template <class T> int emb_vec(const void *p, const void *q, long long width, long long stride) {
-  for (int bytes = 16; bytes > (int)sizeof(T); bytes = bytes == 16 && sizeof(T) == 2 ? 4 : (int)sizeof(T)) {
+  for (int bytes = 16; bytes > (int)sizeof(T); bytes /= 2) {
     const int vec = bytes / (int)sizeof(T);
     if ((uintptr_t)p % bytes == 0 && (uintptr_t)q % bytes == 0 && width % vec == 0 && stride % vec == 0) return vec;
   }
   return 1;
+}
+
+// f(std::integral_constant<int, vec>) for the vec that emb_vec gave.
+template <class T, class F> int emb_with_vec(int vec, F f) {
+  constexpr int most = 16 / (int)sizeof(T);
+  if (vec == most) return f(std::integral_constant<int, most>());
+  if constexpr (most >= 4)
+    if (vec == most / 2) return f(std::integral_constant<int, most / 2>());
+  if constexpr (most >= 8)
+    if (vec == most / 4) return f(std::integral_constant<int, most / 4>());
+  return f(std::integral_constant<int, 1>());
 }
 
 template <class T, class I, int VEC>
@@ -641,12 +693,9 @@ int emb_launch(const T *w, int64_t rows, int64_t width, int64_t w_stride, const 
 template <class T, class I>
 int run_emb(const void *w, int64_t rows, int64_t width, int64_t w_stride, const void *ids, int64_t n, double scale,
             void *out) {
-  const int vec = emb_vec<T>(w, out, width, w_stride);
-  if (vec * sizeof(T) == 16)
-    return emb_launch<T, I, 16 / (int)sizeof(T)>((const T *)w, rows, width, w_stride, (const I *)ids, n, scale, (T *)out);
-  if constexpr (sizeof(T) == 2)
-    if (vec == 2) return emb_launch<T, I, 2>((const T *)w, rows, width, w_stride, (const I *)ids, n, scale, (T *)out);
-  return emb_launch<T, I, 1>((const T *)w, rows, width, w_stride, (const I *)ids, n, scale, (T *)out);
+  return emb_with_vec<T>(emb_vec<T>(w, out, width, w_stride), [&](auto vec) {
+    return emb_launch<T, I, decltype(vec)::value>((const T *)w, rows, width, w_stride, (const I *)ids, n, scale, (T *)out);
+  });
 }
 
 // Device memory of one call, from the stream-ordered pool.
@@ -747,20 +796,17 @@ int run_emb_grad(const void *ids_, int64_t n, const void *grad_, int64_t g_strid
   const T *grad = (const T *)grad_;
   T *out = (T *)out_;
   const int vec = emb_vec<T>(grad, out, width, g_stride);
-  constexpr int WIDE = 16 / (int)sizeof(T);
-  if (n <= mmpd::kEmbFew) {
-    if (vec == WIDE) return emb_few<T, I, WIDE>(ids, (unsigned)n, grad, g_stride, rows, width, scale, padding, out);
-    if constexpr (sizeof(T) == 2)
-      if (vec == 2) return emb_few<T, I, 2>(ids, (unsigned)n, grad, g_stride, rows, width, scale, padding, out);
-    return emb_few<T, I, 1>(ids, (unsigned)n, grad, g_stride, rows, width, scale, padding, out);
-  }
+  if (n <= mmpd::kEmbFew)
+    return emb_with_vec<T>(vec, [&](auto v) {
+      return emb_few<T, I, decltype(v)::value>(ids, (unsigned)n, grad, g_stride, rows, width, scale, padding, out);
+    });
   int bits = 1;
   while ((INT64_C(1) << bits) <= rows) ++bits;  // the key `rows` included
   int *err = mmp::device_error_word();
   EmbBuf mem;
   EmbSorted e;
   e.n = (unsigned)n;
-  const size_t np = ((size_t)n + 3) & ~(size_t)3, words = ((size_t)rows + 31) / 32;
+  const size_t np = ((size_t)n + 7) & ~(size_t)7, words = ((size_t)rows + 31) / 32;
   if (n <= mmpd::kEmbCluster) {
     int rc = mem.alloc(np * 8 + words * 4 + 16);
     if (rc) return rc;
@@ -805,10 +851,8 @@ int run_emb_grad(const void *ids_, int64_t n, const void *grad_, int64_t g_strid
     e.keys = kb[cur];
     e.order = ob[cur];
   }
-  if (vec == WIDE) return emb_sum<T, WIDE>(e, grad, g_stride, rows, width, scale, out);
-  if constexpr (sizeof(T) == 2)
-    if (vec == 2) return emb_sum<T, 2>(e, grad, g_stride, rows, width, scale, out);
-  return emb_sum<T, 1>(e, grad, g_stride, rows, width, scale, out);
+  return emb_with_vec<T>(
+      vec, [&](auto v) { return emb_sum<T, decltype(v)::value>(e, grad, g_stride, rows, width, scale, out); });
 }
 
 }  // namespace
