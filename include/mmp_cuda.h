@@ -114,7 +114,8 @@ int mmp_synchronize(void);
  * offset out of range, 5 = gather / scatter / compaction offset or
  * embedding id out of range, 6 = the self-test wait ran out (mmp_selftest_bounded_wait),
  * 8 = a peer's flag did not arrive in mmp_reduce_allranks,
- * mmp_scan_allranks or mmp_allreduce_sum_peer. */
+ * mmp_scan_allranks or mmp_allreduce_sum_peer, 9 = a copy, or another
+ * block's part, did not arrive in mmp_recurrence or mmp_recurrence_grad. */
 int mmp_check_device_error(int *code);
 
 /* ---- timing */

@@ -873,7 +873,11 @@ int rec_dispatch(int dtype, const RecArgs &g) {
   if (g.steps <= (GRAD ? 16 : 32)) {
     const bool states = ((uintptr_t)g.h0 | (uintptr_t)g.seed | (uintptr_t)g.last) % 16 == 0;
     const bool wide = states && rec_aligned(g, nin, nout, 16, mmp_dtype_size(dtype));
-    if (dtype == MMP_FLOAT16) return wide ? rec_short<__half, 8, GRAD, GATED>(g) : rec_short<__half, 1, GRAD, GATED>(g);
+    if (dtype == MMP_FLOAT16) {
+      if (wide) return rec_short<__half, 8, GRAD, GATED>(g);
+      return states && rec_aligned(g, nin, nout, 4, 2) ? rec_short<__half, 2, GRAD, GATED>(g)
+                                                       : rec_short<__half, 1, GRAD, GATED>(g);
+    }
     if (dtype == MMP_FLOAT32) return wide ? rec_short<float, 4, GRAD, GATED>(g) : rec_short<float, 1, GRAD, GATED>(g);
     return wide ? rec_short<double, 2, GRAD, GATED>(g) : rec_short<double, 1, GRAD, GATED>(g);
   }

@@ -202,6 +202,61 @@ def test_recurrence_gate_limits(cp, dt):
     close(got[2].get(), dh0, e0 * UNIT[dt], "float64" if dt == "float64" else "float32")
 
 
+# (outer, steps, inner): rows copied as tensors in blocks alone and in clusters,
+# one wave and several, and as many blocks as take clusters of eight in several
+LONG = [(1, 5000, 256), (3, 2500, 512), (2, 1500, 1000), (40, 200, 512), (6, 1000, 1024), (1, 10800, 1248),
+        (1, 700, 4000)]
+
+
+@pytest.mark.parametrize("dt,gated", [("float16", True), ("float32", False), ("float32", True), ("float64", True)])
+@pytest.mark.parametrize("shape", LONG)
+def test_recurrence_long(cp, dt, gated, shape):
+    if dt == "float64" and shape[1] * shape[0] * shape[2] > 2 ** 22:
+        shape = (shape[0], shape[1] // 8, shape[2])
+    a, x, h0, g, gs = rec_inputs(shape, dt, gated, shape[1])
+    hs, es, last, el = recurrence(a, x, h0, gated)
+    state = cp.empty(h0.shape, dtype=str(h0.dtype))
+    h = cp.linear_recurrence(cp.array(a), cp.array(x), cp.array(h0), gated=gated, state_out=state)
+    close(h.get(), hs, es * UNIT[dt], dt)
+    close(state.get(), last, el * UNIT[dt], str(state.dtype))
+    del hs, es
+    da, dx, dh0, ea, ex, e0 = recurrence_grad(a, x, h.get(), g, h0, gs, gated)
+    got = cp.linear_recurrence_grad(cp.array(a), cp.array(x), h, cp.array(g), cp.array(h0), gated=gated,
+                                    grad_state=cp.array(gs))
+    close(got[0].get(), da, ea * UNIT[dt], dt)
+    close(got[1].get(), dx, ex * UNIT[dt], dt)
+    close(got[2].get(), dh0, e0 * UNIT[dt], str(h0.dtype))
+
+
+def test_recurrence_decays_above_one(cp):
+    """Spans whose decays multiply past float32's range: a state of zero stays
+    zero, and what is finite step by step is finite."""
+    steps, width = 3000, 64
+    a = np.full((1, steps, width), 2.0, np.float32)
+    x = np.zeros((1, steps, width), np.float32)
+    x[0, -30:, ::2] = 1.0
+    h = cp.linear_recurrence(cp.array(a), cp.array(x)).get()
+    np.testing.assert_array_equal(h[0, :-30], 0)
+    np.testing.assert_array_equal(h[0, :, 1::2], 0)
+    # 2^k - 1: exact up to k = 24; each step after that rounds once, 2^-24 of a
+    # value that its error has grown along with, so six roundings at most
+    want = 2.0 ** np.arange(1, 31) - 1
+    np.testing.assert_array_equal(h[0, -30:-6, 0], want[:24])
+    assert (np.abs(h[0, -6:, 0] - want[24:]) <= 6 * 2.0 ** -24 * want[24:]).all()
+
+
+def test_recurrence_offsets_past_32_bits(cp):
+    """More than 2^31 elements: with decay zero h is x, wherever it lies."""
+    steps, width = (1 << 21) + 37, 1032
+    x = (cp.arange(steps, dtype="int32") % 1021).astype("float16")
+    x = (x.reshape(1, steps, 1) + cp.zeros((1, 1, width), dtype="float16"))
+    a = cp.zeros((1, 1, width), dtype="float16").broadcast_to((1, steps, width))
+    h = cp.linear_recurrence(a, x)
+    assert bool(cp.array_equal(h, x))
+    _, dx, _ = cp.linear_recurrence_grad(a, None, h, x, out=(h, cp.empty(x.shape, dtype="float16")))
+    assert bool(cp.array_equal(dx, x))
+
+
 def test_recurrence_nan_stays_in_its_chain(cp):
     a, x, h0, g, _ = rec_inputs((2, 300, 70), "float32", True, 3)
     x[0, 100, 7] = np.nan
@@ -472,6 +527,28 @@ def test_embedding_shapes_views_and_empty(cp):
     cp.synchronize()
 
 
+def test_embedding_offsets_past_32_bits(cp):
+    """Tables of more than 2^31 elements, few tokens and many."""
+    rows, width = (1 << 21) + 5, 1032
+    w = cp.zeros((rows, width), dtype="float16")
+    w[rows - 1] = 3
+    w[rows - 2, 1000:] = 5
+    ids = np.array([rows - 1, 0, rows - 2, rows - 1], np.int64)
+    got = cp.embedding(w, cp.array(ids), 2.0).get()
+    want = np.zeros((4, width), np.float16)
+    want[[0, 3]] = 6
+    want[2, 1000:] = 10
+    np.testing.assert_array_equal(got, want)
+    for n in (4, 4000):
+        many = np.resize(ids, n)
+        out = cp.embedding_grad(cp.array(many), cp.ones((n, width), dtype="float16"), rows, out=w)
+        count = np.bincount(many, minlength=rows)
+        assert float(cp.sum(out[1:rows - 2].astype("float32")).get()) == 0
+        np.testing.assert_array_equal(out[[0, rows - 2, rows - 1]].get(),
+                                      np.repeat(count[[0, rows - 2, rows - 1], None], width, 1))
+    cp.synchronize()
+
+
 def test_embedding_ids_out_of_range(cp):
     """A bad id gives zeros (lookup) or adds nothing (gradient), and the next
     synchronize raises once."""
@@ -677,3 +754,112 @@ def test_decode_follows_training(cp):
         i = cp.array(ids[:, t:t + 1])
         h = cp.linear_recurrence(cp.embedding(G, i), cp.embedding(T, i), s, gated=True, state_out=s)
         close(h.get()[:, 0], hs[:, t], es[:, t] * UNIT["float16"], "float16")
+
+
+def test_from_several_threads(cp):
+    """Calls from several threads at once (each gets its own results)."""
+    import threading
+
+    from macmetalpy_b200 import _cuda_backend as cb
+
+    rng = np.random.default_rng(9)
+    work = []
+    for k in range(4):
+        a, x, _, _, _ = rec_inputs((2, 400 + k, 96), "float32", True, 40 + k)
+        ids, g = rng.integers(0, 3000, 5000 + k), rng.standard_normal((5000 + k, 24)).astype(np.float32)
+        work.append((a, x, ids, g))
+
+    def one(w, to):
+        a, x, ids, g = w
+        cb.check(cb.lib.mmp_init(cb.CudaBackend().device))  # the device of a new thread
+        for _ in range(5):
+            h = cp.linear_recurrence(cp.array(a), cp.array(x), gated=True)
+            d = cp.embedding_grad(cp.array(ids), cp.array(g), 3000)
+            _, n = cp.clip_by_global_norm([h, d], 1.0)
+            to.append((h.get(), d.get(), float(n)))
+
+    alone, together = [[] for _ in work], [[] for _ in work]
+    for w, to in zip(work, alone):
+        one(w, to)
+    threads = [threading.Thread(target=one, args=(w, to)) for w, to in zip(work, together)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for p, q in zip(alone, together):
+        assert len(q) == 5
+        for r in q:
+            np.testing.assert_array_equal(r[0], p[0][0])
+            np.testing.assert_array_equal(r[1], p[0][1])
+            assert r[2] == p[0][2]
+
+
+CAPTURE = """
+import sys
+sys.path.insert(0, {repo!r})
+import ctypes
+import numpy as np
+import torch
+import macmetalpy_b200 as cp
+from macmetalpy_b200 import _cuda_backend as cb
+cp.synchronize()
+stream = torch.cuda.Stream()
+cb.check(cb.lib.mmp_set_stream(ctypes.c_void_p(stream.cuda_stream)))
+rng = np.random.default_rng(0)
+f = lambda *s, dt="float32": cp.array(rng.standard_normal(s).astype(dt))
+z, x, g = f(2, 700, 128, dt="float16"), f(2, 700, 128, dt="float16"), f(2, 700, 128, dt="float16")
+h, da, dx = (cp.empty((2, 700, 128), dtype="float16") for _ in range(3))
+s = cp.zeros((2, 128), dtype="float32")
+ids = [cp.array(rng.integers(0, 500, n)) for n in (300, 3000)]
+gr = [f(n, 40) for n in (300, 3000)]
+dw = [cp.empty((500, 40), dtype="float32") for _ in ids]
+e = cp.empty((300, 40), dtype="float32")
+clipped = [cp.empty((500, 40), dtype="float32") for _ in ids]
+norm = cp.empty((), dtype="float32")
+def step():
+    cp.linear_recurrence(z, x, s, gated=True, out=h, state_out=s)
+    cp.linear_recurrence_grad(z, x, h, g, gated=True, out=(da, dx))
+    for i, r, d in zip(ids, gr, dw):
+        cp.embedding_grad(i, r, 500, 2.0, out=d)
+    cp.embedding(dw[0], ids[0], 0.5, out=e)
+    cp.clip_by_global_norm(dw, 1.0, out=clipped, norm_out=norm)
+def results():
+    return [a.get() for a in (h, da, dx, s, e, norm, *dw, *clipped)]
+step(); step(); cp.synchronize()
+graphs = []
+for _ in range(2):
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        step()
+    graphs.append(graph)
+for k in range(4):
+    new = [rng.standard_normal(a.shape).astype(a.dtype) for a in (z, x, g, *gr)]
+    for a, v in zip((z, x, g, *gr), new):
+        a.set(v)
+    for i in ids:
+        i.set(rng.integers(0, 500, i.shape))
+    s0 = rng.standard_normal((2, 128)).astype("float32")
+    s.set(s0); cp.synchronize()
+    step(); want = results()
+    s.set(s0); cp.synchronize()
+    with torch.cuda.stream(stream):
+        graphs[k % 2].replay()
+    torch.cuda.synchronize()
+    for p, q in zip(want, results()):
+        np.testing.assert_array_equal(p, q)
+cp.synchronize()
+print("captured")
+"""
+
+
+def test_captured_and_replayed(cp):
+    """Every operator captured into two graphs on a foreign stream and replayed
+    on new inputs gives what the plain calls give (a process of its own: the
+    library keeps the stream it is given)."""
+    import os
+    import subprocess
+    import sys
+
+    repo = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    p = subprocess.run([sys.executable, "-c", CAPTURE.format(repo=repo)], capture_output=True, text=True, timeout=300)
+    assert p.returncode == 0 and "captured" in p.stdout, p.stdout + p.stderr
