@@ -259,11 +259,13 @@ __global__ void __launch_bounds__(256) emb_grad_few(const I *__restrict__ ids, u
 // ---- the sort of up to kEmbCluster tokens by one cluster, beside the zeros.
 constexpr int kSortThreads = 1024, kSortRanks = 8, kSortItems = 8;
 constexpr unsigned kEmbCluster = kSortThreads * kSortRanks * kSortItems;  // 65536
+constexpr int kSortBits = 9, kSortBins = 1 << kSortBits;  // of a digit at most
 struct EmbSortSmem {
-  unsigned count[32][256];          // a warp's keys of each digit
-  unsigned total[kSortRanks][256];  // each block's
-  unsigned base[256];
-  unsigned sum[8];
+  unsigned short count[32][kSortBins];    // a warp's keys of each digit, then those of the warps before it
+  unsigned total[kSortRanks][kSortBins];  // each block's
+  unsigned local[kSortBins];              // the digit's first place in the block's order
+  unsigned base[kSortBins];               // and in the whole order, for this block's keys
+  unsigned sum[2][kSortBins / 32];
   unsigned long long key[2][1];  // E * 1024 each: id << 32 | token
 };
 
@@ -273,9 +275,27 @@ __device__ __forceinline__ unsigned emb_lanemask_lt() {
   return m;
 }
 
+// Inclusive sums over the first kSortBins threads (s_sum: one word a warp).
+__device__ __forceinline__ unsigned emb_scan_bins(unsigned v, unsigned *s_sum) {
+  const unsigned lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned t = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += t;
+  }
+  if (lane == 31) s_sum[w] = v;
+  asm volatile("bar.sync 1, %0;" ::"n"(kSortBins) : "memory");
+#pragma unroll
+  for (unsigned u = 0; u < kSortBins / 32; ++u)
+    if (u < w) v += s_sum[u];
+  return v;
+}
+
 // Cluster 0 sorts (LSD radix: a block has E * 1024 neighbouring keys in its
-// shared memory, a warp E * 32 of them; keys go to their place in the next
-// pass through the cluster's shared memory).  A key that counts for no row
+// shared memory, a warp E * 32 of them; a pass puts them in the block's order
+// first, so that neighbouring threads then send neighbouring keys to their
+// place in the cluster's shared memory: sent one by one, a pass of 30,000 keys
+// took 13 us).  A key that counts for no row
 // (padding, out of range) is `rows`.  It also marks the ids in the bitmap
 // `seen`.  The other clusters write the zeros of the rows below `zeros`.
 template <class T, class I>
@@ -320,7 +340,7 @@ __global__ void __cluster_dims__(kSortRanks, 1, 1) __launch_bounds__(kSortThread
     const int shift = 32 + pass * digit;
     const unsigned mask = (1u << digit) - 1;
     unsigned long long *from = buf[pass & 1];
-    for (unsigned j = tid; j < 32 * 256; j += kSortThreads) (&s.count[0][0])[j] = 0;
+    for (unsigned j = tid; j < sizeof(s.count) / 4; j += kSortThreads) reinterpret_cast<unsigned *>(s.count)[j] = 0;
     __syncthreads();
     unsigned long long k[kSortItems];
     unsigned at[kSortItems];
@@ -338,31 +358,40 @@ __global__ void __cluster_dims__(kSortRanks, 1, 1) __launch_bounds__(kSortThread
         }
         const unsigned c = valid ? s.count[w][d] : 0u, before = __popc(peers & lt);
         __syncwarp();
-        if (valid && before == 0) s.count[w][d] = c + __popc(peers);
+        if (valid && before == 0) s.count[w][d] = (unsigned short)(c + __popc(peers));
         __syncwarp();
         at[e] = c + before;
       }
     }
     __syncthreads();
-    if (tid < 256) {  // thread = digit: each warp's first place among the block's keys of the digit
-      unsigned c[32], t = 0;
+    // thread = digit: each warp's first place among the block's keys of the
+    // digit, the digit's first place in the block
+    unsigned mine = 0, inc = 0;
+    if (tid < kSortBins) {
+      unsigned short c[32];
 #pragma unroll
       for (int v = 0; v < 32; ++v) c[v] = s.count[v][tid];
 #pragma unroll
       for (int v = 0; v < 32; ++v) {
-        s.count[v][tid] = t;
-        t += c[v];
+        s.count[v][tid] = (unsigned short)mine;
+        mine += c[v];
       }
-      for (int r = 0; r < kSortRanks; ++r) *cl.map_shared_rank(&s.total[rank][tid], r) = t;
+      for (int r = 0; r < kSortRanks; ++r) *cl.map_shared_rank(&s.total[rank][tid], r) = mine;
+      inc = emb_scan_bins(mine, s.sum[0]);
+      s.local[tid] = inc - mine;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < kSortItems; ++e) {
+      if (e < items && rank * tile + place + e * 32 < n) {
+        const unsigned d = (unsigned)(k[e] >> shift) & mask;
+        const unsigned q = s.local[d] + s.count[w][d] + at[e];
+        if (q < tile) from[q] = k[e];
+        else atomicExch(err, 4);  // inconsistent counts: report, never write out of bounds
+      }
     }
     cl.sync();
-    if (pass == 0) {  // the bitmap is zeroed
-#pragma unroll
-      for (int e = 0; e < kSortItems; ++e)
-        if (e < items)
-          emb_mark(seen, (unsigned)(k[e] >> 32), rank * tile + place + e * 32 < n && (k[e] >> 32) < (unsigned long long)rows);
-    }
-    if (tid < 256) {
+    if (tid < kSortBins) {
       unsigned all = 0, below = 0;
 #pragma unroll
       for (int r = 0; r < kSortRanks; ++r) {
@@ -370,36 +399,33 @@ __global__ void __cluster_dims__(kSortRanks, 1, 1) __launch_bounds__(kSortThread
         if (r < (int)rank) below += t;
         all += t;
       }
-      unsigned inc = all;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const unsigned t = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += t;
-      }
-      if (lane == 31) s.sum[w] = inc;
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      unsigned pre = 0;
-#pragma unroll
-      for (unsigned v = 0; v < 8; ++v)
-        if (v < w) pre += s.sum[v];
-      s.base[tid] = pre + inc - all + below;
+      s.base[tid] = emb_scan_bins(all, s.sum[1]) - all + below;
     }
     __syncthreads();
     const bool final = pass + 1 == passes;
     unsigned long long *to = buf[(pass & 1) ^ 1];
+    const unsigned have = n > rank * tile ? (n - rank * tile < tile ? n - rank * tile : tile) : 0;
 #pragma unroll
     for (int e = 0; e < kSortItems; ++e) {
-      if (e < items && rank * tile + place + e * 32 < n) {
-        const unsigned d = (unsigned)(k[e] >> shift) & mask;
-        const unsigned dst = s.base[d] + s.count[w][d] + at[e];
-        if (dst >= n) {  // inconsistent counts: report, never write out of bounds
+      const unsigned j = e * kSortThreads + tid;
+      if (final && e < items) {
+        // the block's keys are in order now: the first of each id in the warp marks it
+        const unsigned id = j < have ? (unsigned)(from[j] >> 32) : 0xffffffffu;
+        const unsigned left = __shfl_up_sync(0xffffffffu, id, 1);
+        if (id < (unsigned)rows && (lane == 0 || left != id)) atomicOr(&seen[id >> 5], 1u << (id & 31));
+      }
+      if (j < have) {
+        const unsigned long long key = from[j];
+        const unsigned d = (unsigned)(key >> shift) & mask;
+        const unsigned dst = s.base[d] + j - s.local[d];
+        if (dst >= n) {
           atomicExch(err, 4);
         } else if (final) {
-          keys[dst] = (unsigned)(k[e] >> 32);
-          order[dst] = (unsigned)k[e];
+          keys[dst] = (unsigned)(key >> 32);
+          order[dst] = (unsigned)key;
         } else {
           const unsigned r = dst / tile;
-          *cl.map_shared_rank(&to[dst - r * tile], r) = k[e];
+          *cl.map_shared_rank(&to[dst - r * tile], r) = key;
         }
       }
     }
@@ -815,7 +841,7 @@ int run_emb_grad(const void *ids_, int64_t n, const void *grad_, int64_t g_strid
     e.seen = e.order + np;
     e.runs = e.seen + words;
     const int items = (int)((n + mmpd::kSortThreads * mmpd::kSortRanks - 1) / (mmpd::kSortThreads * mmpd::kSortRanks));
-    const int passes = (bits + 7) / 8, digit = (bits + passes - 1) / passes;
+    const int passes = (bits + mmpd::kSortBits - 1) / mmpd::kSortBits, digit = (bits + passes - 1) / passes;
     // the sort takes some 10 us: as many zeros beside it as are written in that time
     const int64_t row = width * (int64_t)sizeof(T), most = (int64_t)48 << 20;
     e.zeros = (unsigned)(rows * row < most ? rows : most / row);
