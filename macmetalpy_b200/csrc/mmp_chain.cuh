@@ -1,0 +1,40 @@
+// Kernels that follow one another on the library stream: a kernel launched by
+// launch_after may be set up while the one before it in the stream ends.  It
+// calls chain_wait before it touches memory, which waits until that one is
+// done and its writes are there, and chain_next to let the one behind it be
+// set up in turn.
+#pragma once
+#include <cuda_runtime.h>
+
+#include "mmp_internal.h"
+
+namespace mmpd {
+
+__device__ __forceinline__ void chain_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void chain_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+}  // namespace mmpd
+
+namespace mmp {
+
+// `ranks`: blocks a cluster (1: none, or the kernel's own).
+template <class... P, class... A>
+int launch_after(void (*fn)(P...), dim3 grid, dim3 block, size_t smem, int ranks, const A &...args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream();
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = (unsigned)ranks;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = ranks > 1 ? 2 : 1;
+  MMP_CUDA_TRY(cudaLaunchKernelEx(&cfg, fn, P(args)...));
+  return MMP_OK;
+}
+
+}  // namespace mmp

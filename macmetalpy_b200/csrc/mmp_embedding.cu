@@ -26,6 +26,7 @@
 
 #include <type_traits>
 
+#include "mmp_chain.cuh"
 #include "mmp_device.cuh"
 #include "mmp_internal.h"
 
@@ -46,6 +47,8 @@ __global__ void __launch_bounds__(256) emb_kernel(const T *__restrict__ w, long 
   typedef typename EmbAcc<T>::type S;
   typedef EmbVec<T, VEC> V;
   const unsigned i0 = blockIdx.x * (256u * U) + threadIdx.x;
+  chain_wait();
+  chain_next();
   unsigned col[U];
   long long id[U];
 #pragma unroll
@@ -172,9 +175,6 @@ __device__ __forceinline__ void emb_mark(unsigned *seen, unsigned id, bool want)
   if (~*(volatile unsigned *)(seen + word) & bits) atomicOr(seen + word, bits);
 }
 
-__device__ __forceinline__ void emb_wait_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void emb_next_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-
 // ---- few tokens, one launch.  Blocks [0, n): token blockIdx.x, if it is the
 // first of its id, adds all of them in the order of n.  The others: zeros.
 template <class T, class I, int VEC>
@@ -187,6 +187,8 @@ __global__ void __launch_bounds__(256) emb_grad_few(const I *__restrict__ ids, u
   __shared__ unsigned s_buf[kEmbFew];  // the list of tokens, or the bitmap
   __shared__ unsigned s_sum[8];
   const unsigned tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  chain_wait();
+  chain_next();
   if (blockIdx.x >= n) {
     emb_zero_share<T, I>(ids, n, rows, padding, blockIdx.x - n, gridDim.x - n, kEmbFewBits, width, out, s_buf, err);
     return;
@@ -305,7 +307,8 @@ __global__ void __cluster_dims__(kSortRanks, 1, 1) __launch_bounds__(kSortThread
                     T *__restrict__ out, unsigned zeros, unsigned bits, unsigned *__restrict__ seen,
                     unsigned *__restrict__ runs, int *err) {
   extern __shared__ __align__(16) unsigned char s_raw[];
-  emb_next_may_start();
+  chain_wait();
+  chain_next();
   if (blockIdx.x >= kSortRanks) {
     emb_zero_share<T, I>(ids, n, zeros, padding, blockIdx.x - kSortRanks, gridDim.x - kSortRanks, bits, width, out,
                          (unsigned *)s_raw, nullptr);
@@ -474,8 +477,8 @@ __global__ void __launch_bounds__(256) emb_sum_kernel(const unsigned *__restrict
                                                       unsigned zeros_end, unsigned unit, unsigned zero_blocks) {
   typedef typename EmbAcc<T>::type S;
   typedef EmbVec<T, VEC> V;
-  emb_wait_before();
-  emb_next_may_start();
+  chain_wait();
+  chain_next();
   if (blockIdx.x < zero_blocks) {  // the zeros of the rows [zeros, zeros_end)
     emb_zero_marked(seen, zeros, zeros_end, width, out, unit,
                     (blockIdx.y * zero_blocks + blockIdx.x) * 8 + threadIdx.x / 32, gridDim.y * zero_blocks * 8);
@@ -605,7 +608,7 @@ __global__ void __launch_bounds__(256) emb_join_kernel(unsigned width, typename 
   typedef typename EmbAcc<T>::type S;
   typedef EmbVec<S, JV> V;
   __shared__ V s_part[8][32];
-  emb_wait_before();
+  chain_wait();
   if (blockIdx.x >= join_blocks) {  // the zeros of the rows from `zeros` on
     const unsigned blocks = gridDim.x - join_blocks;
     emb_zero_marked(seen, zeros, rows, width, out, unit,
@@ -705,13 +708,11 @@ int emb_launch(const T *w, int64_t rows, int64_t width, int64_t w_stride, const 
     const unsigned total = (unsigned)(m * per);
     int *err = mmp::device_error_word();
     // four vectors a thread where that leaves every SM its blocks
-    if (total >= 1024u * 4 * (unsigned)mmp::sm_count())
-      mmpd::emb_kernel<T, I, VEC, 4><<<(total + 1023) / 1024, 256, 0, mmp::stream()>>>(
-          w, rows, emb_div((unsigned)per), w_stride, ids + r, total, (S)scale, out + r * width, err);
-    else
-      mmpd::emb_kernel<T, I, VEC, 1><<<(total + 255) / 256, 256, 0, mmp::stream()>>>(
-          w, rows, emb_div((unsigned)per), w_stride, ids + r, total, (S)scale, out + r * width, err);
-    MMP_LAUNCH_CHECK("embedding");
+    const bool four = total >= 1024u * 4 * (unsigned)mmp::sm_count();
+    const int rc = mmp::launch_after(four ? mmpd::emb_kernel<T, I, VEC, 4> : mmpd::emb_kernel<T, I, VEC, 1>,
+                                     four ? (total + 1023) / 1024 : (total + 255) / 256, 256, 0, 1, w, rows,
+                                     emb_div((unsigned)per), w_stride, ids + r, total, (S)scale, out + r * width, err);
+    if (rc) return rc;
   }
   return MMP_OK;
 }
@@ -742,55 +743,45 @@ int emb_few(const I *ids, unsigned n, const T *grad, int64_t g_stride, int64_t r
   // a block a token, and eight an SM for the zeros while they have a 64 KB each
   const int64_t most = (int64_t)mmp::sm_count() * 8, want = rows * width * (int64_t)sizeof(T) / 65536 + 1;
   const unsigned zero = (unsigned)(want < most ? want : most);
-  mmpd::emb_grad_few<T, I, VEC><<<n + zero, 256, 0, mmp::stream()>>>(
-      ids, n, grad, g_stride, rows, (unsigned)width, (typename mmpd::EmbAcc<T>::type)scale, padding, out,
-      mmp::device_error_word());
-  MMP_LAUNCH_CHECK("embedding_grad");
-  return MMP_OK;
+  return mmp::launch_after(mmpd::emb_grad_few<T, I, VEC>, n + zero, 256, 0, 1, ids, n, grad, g_stride, rows, (unsigned)width,
+                           (typename mmpd::EmbAcc<T>::type)scale, padding, out, mmp::device_error_word());
 }
 
-// A launch that may begin while the kernel before it in the stream ends (it
-// waits for that one itself).
-template <class... P, class... A>
-int emb_launch_after(void (*fn)(P...), dim3 grid, A... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(256);
-  cfg.stream = mmp::stream();
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  MMP_CUDA_TRY(cudaLaunchKernelEx(&cfg, fn, P(args)...));
-  return MMP_OK;
+// How the sums are shared out.
+struct EmbShares {
+  unsigned lanes, slices, groups, share, shares;
+};
+EmbShares emb_shares(unsigned n, int64_t width, int vec) {
+  EmbShares r;
+  r.lanes = 1;
+  while (r.lanes < 256 && r.lanes * vec < width) r.lanes *= 2;
+  r.slices = (unsigned)((width + (int64_t)r.lanes * vec - 1) / ((int64_t)r.lanes * vec));
+  r.groups = 256 / r.lanes;
+  // shares of 32 tokens: fewer where that leaves SMs without blocks, more
+  // where it makes more than sixteen blocks an SM (each share may leave two
+  // parts to join)
+  const unsigned sms = (unsigned)mmp::sm_count();
+  r.share = 32;
+  auto blocks = [&] { return ((uint64_t)n + r.share - 1) / r.share * r.slices / r.groups; };
+  while (r.share > 8 && blocks() < 4u * sms) r.share /= 2;
+  while (blocks() > 16u * sms) r.share *= 2;
+  r.shares = (n + r.share - 1) / r.share;
+  return r;
 }
 
 struct EmbSorted {
   unsigned *keys, *order, *runs, *seen;
+  mmpd::EmbRun *list;
+  void *part;
   unsigned n, zeros;  // rows below `zeros` have theirs
+  EmbShares sh;
 };
 
 template <class T, int VEC>
 int emb_sum(const EmbSorted &e, const T *grad, int64_t g_stride, int64_t rows, int64_t width, double scale, T *out) {
   typedef typename mmpd::EmbAcc<T>::type S;
-  const unsigned n = e.n;
-  unsigned lanes = 1;
-  while (lanes < 256 && lanes * VEC < width) lanes *= 2;
-  const unsigned slices = (unsigned)((width + (int64_t)lanes * VEC - 1) / ((int64_t)lanes * VEC)), groups = 256 / lanes;
-  // shares of 32 tokens: fewer where that leaves SMs without blocks, more
-  // where it makes more than sixteen blocks an SM (each share may leave two
-  // parts to join)
-  unsigned share = 32;
-  auto blocks = [&] { return ((uint64_t)n + share - 1) / share * slices / groups; };
-  while (share > 8 && blocks() < 4u * (unsigned)mmp::sm_count()) share /= 2;
-  while (blocks() > 16u * (unsigned)mmp::sm_count()) share *= 2;
-  const unsigned shares = (n + share - 1) / share;
-  EmbBuf part;
-  const size_t np = (size_t)shares * 2 * width * sizeof(S);
-  int rc = part.alloc(np + shares * sizeof(mmpd::EmbRun));
-  if (rc) return rc;
-  mmpd::EmbRun *list = (mmpd::EmbRun *)((char *)part.p + np);
+  const unsigned n = e.n, lanes = e.sh.lanes, slices = e.sh.slices, groups = e.sh.groups, share = e.sh.share,
+                 shares = e.sh.shares;
   // Beside them two blocks an SM that write zeros, 8 KB of rows a warp at a
   // time; the last 24 MB are left for the joining kernel, which waits for
   // memory some 6 us and moves next to nothing.
@@ -803,16 +794,16 @@ int emb_sum(const EmbSorted &e, const T *grad, int64_t g_stride, int64_t rows, i
     return (unsigned)(want < most ? want : most);
   };
   const unsigned zero_blocks = zero_grid(e.zeros, zeros_end, 2 * (unsigned)mmp::sm_count());
-  rc = emb_launch_after(mmpd::emb_sum_kernel<T, VEC>, dim3(zero_blocks + (shares + groups - 1) / groups, slices), e.keys,
+  const int rc = mmp::launch_after(mmpd::emb_sum_kernel<T, VEC>, dim3(zero_blocks + (shares + groups - 1) / groups, slices), 256, 0, 1, e.keys,
                         e.order, n, share, shares, lanes, grad, g_stride, (unsigned)rows, (unsigned)width, (S)scale, out,
-                        (S *)part.p, e.runs, list, e.seen, e.zeros, zeros_end, unit, zero_blocks);
+                        (S *)e.part, e.runs, e.list, e.seen, e.zeros, zeros_end, unit, zero_blocks);
   if (rc) return rc;
   constexpr int JV = VEC >= 4 ? 4 : 1;
   const unsigned cols = (unsigned)((width + 32 * JV - 1) / (32 * JV));
   const unsigned join = shares < 128 ? shares : 128, slots = cols < 32 ? cols : 32;
   const unsigned last = zero_grid(zeros_end, (unsigned)rows, (4 * (unsigned)mmp::sm_count() + slots - 1) / slots);
-  return emb_launch_after(mmpd::emb_join_kernel<T, JV>, dim3(join + last, slots), (unsigned)width, (S)scale,
-                          (const S *)part.p, e.runs, list, out, e.seen, zeros_end, (unsigned)rows, unit, join);
+  return mmp::launch_after(mmpd::emb_join_kernel<T, JV>, dim3(join + last, slots), 256, 0, 1, (unsigned)width, (S)scale,
+                          (const S *)e.part, e.runs, e.list, out, e.seen, zeros_end, (unsigned)rows, unit, join);
 }
 
 template <class T, class I>
@@ -832,18 +823,25 @@ int run_emb_grad(const void *ids_, int64_t n, const void *grad_, int64_t g_strid
   EmbBuf mem;
   EmbSorted e;
   e.n = (unsigned)n;
+  e.sh = emb_shares(e.n, width, vec);
+  // keys, order (a second time each for sort_pairs), parts, list, bitmap, count
+  const bool cluster = n <= mmpd::kEmbCluster;
   const size_t np = ((size_t)n + 7) & ~(size_t)7, words = ((size_t)rows + 31) / 32;
-  if (n <= mmpd::kEmbCluster) {
-    int rc = mem.alloc(np * 8 + words * 4 + 16);
-    if (rc) return rc;
-    e.keys = (unsigned *)mem.p;
-    e.order = e.keys + np;
-    e.seen = e.order + np;
-    e.runs = e.seen + words;
+  const size_t parts = (size_t)e.sh.shares * 2 * width * sizeof(typename mmpd::EmbAcc<T>::type);
+  const size_t sorted = np * (cluster ? 8 : 16), lists = ((size_t)e.sh.shares * sizeof(mmpd::EmbRun) + 15) / 16 * 16;
+  int rc = mem.alloc(sorted + (parts + 15) / 16 * 16 + lists + words * 4 + 16);
+  if (rc) return rc;
+  e.keys = (unsigned *)mem.p;
+  e.order = e.keys + np;
+  e.part = (char *)mem.p + sorted;
+  e.list = (mmpd::EmbRun *)((char *)e.part + (parts + 15) / 16 * 16);
+  e.seen = (unsigned *)((char *)e.list + lists);
+  e.runs = e.seen + words;
+  if (cluster) {
     const int items = (int)((n + mmpd::kSortThreads * mmpd::kSortRanks - 1) / (mmpd::kSortThreads * mmpd::kSortRanks));
     const int passes = (bits + mmpd::kSortBits - 1) / mmpd::kSortBits, digit = (bits + passes - 1) / passes;
     // the sort takes some 10 us: as many zeros beside it as are written in that time
-    const int64_t row = width * (int64_t)sizeof(T), most = (int64_t)48 << 20;
+    const int64_t row = width * (int64_t)sizeof(T), most = (int64_t)32 << 20;
     e.zeros = (unsigned)(rows * row < most ? rows : most / row);
     // one block an SM in clusters of eight, with 64 KB of zeros each at least
     const int64_t all = mmp::sm_count() / mmpd::kSortRanks - 1;
@@ -855,17 +853,12 @@ int run_emb_grad(const void *ids_, int64_t n, const void *grad_, int64_t g_strid
     if (smem < seen) smem = seen;
     auto fn = mmpd::emb_sort_kernel<T, I>;
     MMP_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    fn<<<clusters * mmpd::kSortRanks, mmpd::kSortThreads, smem, mmp::stream()>>>(
-        ids, (unsigned)n, rows, padding, items, passes, digit, e.keys, e.order, (unsigned)width, out, e.zeros,
-        (unsigned)(seen * 8), e.seen, e.runs, err);
-    MMP_LAUNCH_CHECK("embedding_grad sort");
-  } else {
-    int rc = mem.alloc(np * 16 + words * 4 + 16);
+    rc = mmp::launch_after(fn, dim3(clusters * mmpd::kSortRanks), mmpd::kSortThreads, smem, 1, ids, (unsigned)n, rows, padding,
+                          items, passes, digit, e.keys, e.order, (unsigned)width, out, e.zeros, (unsigned)(seen * 8),
+                          e.seen, e.runs, err);
     if (rc) return rc;
-    unsigned *const kb[2] = {(unsigned *)mem.p, (unsigned *)mem.p + np};
-    unsigned *const ob[2] = {kb[1] + np, kb[1] + 2 * np};
-    e.seen = ob[1] + np;
-    e.runs = e.seen + words;
+  } else {
+    unsigned *const kb[2] = {e.keys, e.keys + 2 * np}, *const ob[2] = {e.order, e.order + 2 * np};
     e.zeros = 0;
     MMP_CUDA_TRY(cudaMemsetAsync(e.seen, 0, words * 4 + 4, mmp::stream()));
     mmpd::emb_prep_kernel<I><<<mmp::sm_count() * 2, 256, 0, mmp::stream()>>>(ids, (unsigned)n, rows, padding, kb[0],

@@ -13,6 +13,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include "mmp_chain.cuh"
 #include "mmp_device.cuh"
 #include "mmp_internal.h"
 
@@ -102,6 +103,8 @@ template <int N>
 __global__ void __launch_bounds__(kNormThreads, 4) norm_sum_kernel(const __grid_constant__ NormTable<N> t,
                                                                    double *partial) {
   double acc = 0.0;
+  chain_wait();
+  chain_next();
   for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
     const NormEntry &e = norm_find(t, c);
     const long long at = (long long)(c - e.first) * kNormChunk;
@@ -156,6 +159,8 @@ template <int N>
 __global__ void __launch_bounds__(kNormThreads, 4) norm_scale_kernel(const __grid_constant__ NormTable<N> t,
                                                                   const double *partial, int npartial, double max_norm,
                                                                   int norm_f64, void *norm_out) {
+  chain_wait();
+  chain_next();
   const double norm = norm_total(partial, npartial);
   if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) {
     if (norm_f64) *(double *)norm_out = norm;
@@ -240,10 +245,10 @@ extern "C" int mmp_global_norm(int64_t count, const int *dtypes, const void *con
     rc = norm_fill(t, &at, count, dtypes, x, y, sizes);
     if (rc || !t.chunks) continue;
     const int grid = (int)(t.chunks < most ? t.chunks : most);
-    if (t.count <= kNormFew)
-      mmpd::norm_sum_kernel<<<grid, mmpd::kNormThreads, 0, st>>>(norm_few(t), partial + npartial);
-    else
-      mmpd::norm_sum_kernel<<<grid, mmpd::kNormThreads, 0, st>>>(t, partial + npartial);
+    rc = t.count <= kNormFew ? mmp::launch_after(mmpd::norm_sum_kernel<kNormFew>, grid, mmpd::kNormThreads, 0, 1,
+                                                 norm_few(t), partial + npartial)
+                             : mmp::launch_after(mmpd::norm_sum_kernel<kNormTable>, grid, mmpd::kNormThreads, 0, 1, t,
+                                                 partial + npartial);
     npartial += grid;
   }
   // with one table the one just filled serves both kernels
@@ -256,15 +261,12 @@ extern "C" int mmp_global_norm(int64_t count, const int *dtypes, const void *con
     const int grid = (int)(t.chunks < 1 ? 1 : t.chunks < most ? t.chunks : most);
     void *const to = first ? norm : nullptr;
     const int f64 = norm_dtype == MMP_FLOAT64;
-    if (t.count <= kNormFew)
-      mmpd::norm_scale_kernel<<<grid, mmpd::kNormThreads, 0, st>>>(norm_few(t), partial, npartial, max_norm, f64, to);
-    else
-      mmpd::norm_scale_kernel<<<grid, mmpd::kNormThreads, 0, st>>>(t, partial, npartial, max_norm, f64, to);
+    rc = t.count <= kNormFew ? mmp::launch_after(mmpd::norm_scale_kernel<kNormFew>, grid, mmpd::kNormThreads, 0, 1,
+                                                 norm_few(t), partial, npartial, max_norm, f64, to)
+                             : mmp::launch_after(mmpd::norm_scale_kernel<kNormTable>, grid, mmpd::kNormThreads, 0, 1, t,
+                                                 partial, npartial, max_norm, f64, to);
     first = false;
   }
-  const cudaError_t le = cudaGetLastError();
   cudaFreeAsync(partial, st);
-  if (rc) return rc;
-  if (le != cudaSuccess) return mmp::cuda_error(le, "global_norm");
-  return MMP_OK;
+  return rc;
 }

@@ -33,6 +33,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include "mmp_chain.cuh"
 #include "mmp_device.cuh"
 #include "mmp_internal.h"
 
@@ -272,6 +273,8 @@ __global__ void __launch_bounds__(32 * (kRecWarps + 1), 2) rec_kernel(
   // (tensor copies go to multiples of 128 bytes)
   const unsigned skew = (unsigned)(-(int)__cvta_generic_to_shared(s_ring)) & 127u;
   V *const ring = reinterpret_cast<V *>(s_ring + skew) + (size_t)w * g.stages * (NA * N * 32) + lane;
+  chain_wait();
+  chain_next();
   const int span = ranks * warps * N;  // steps of the cluster
   const int mine = (rank * warps + w) * N;
   if (w == warps) {
@@ -643,6 +646,8 @@ __global__ void __launch_bounds__(128) rec_short_kernel(const __grid_constant__ 
     }
   };
   S s[VEC];
+  chain_wait();
+  chain_next();
   states(g.seed, s);
   for (int k0 = 0; k0 < g.steps; k0 += B) {
     V raw[B][NA];
@@ -722,21 +727,8 @@ int rec_launch(const RecArgs &g, const mmpd::RecMaps<COPY> &maps, unsigned block
   auto fn = mmpd::rec_kernel<T, VEC, COPY, GRAD, GATED, CLUSTER>;
   if (smem > 16 * 1024)  // together with the static part this can pass the default 48 KB
     MMP_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(blocks * ranks);
-  cfg.blockDim = dim3(32, g.warps + 1);  // and the joining warp
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = mmp::stream();
-  cudaLaunchAttribute at[1];
-  if (CLUSTER) {
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned)ranks;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-  }
-  MMP_CUDA_TRY(cudaLaunchKernelEx(&cfg, fn, g, maps));
-  return MMP_OK;
+  // the composing warps and the joining one
+  return mmp::launch_after(fn, blocks * ranks, dim3(32, g.warps + 1), smem, ranks, g, maps);
 }
 
 // Byte strides of the second and third axis of a tensor map, as its
@@ -857,9 +849,7 @@ template <class T, int VEC, bool GRAD, bool GATED>
 int rec_short(const RecArgs &g) {
   const long long blocks = (g.outer * (g.inner / VEC) + 127) / 128;
   if (blocks > INT32_MAX) return mmp::set_error(MMP_E_ARG, "recurrence: too many chains");
-  mmpd::rec_short_kernel<T, VEC, GRAD, GATED><<<(unsigned)blocks, 128, 0, mmp::stream()>>>(g);
-  MMP_LAUNCH_CHECK("recurrence");
-  return MMP_OK;
+  return mmp::launch_after(mmpd::rec_short_kernel<T, VEC, GRAD, GATED>, (unsigned)blocks, 128, 0, 1, g);
 }
 
 template <bool GRAD, bool GATED>
