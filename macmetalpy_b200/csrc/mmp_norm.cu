@@ -10,6 +10,9 @@
 // it to the device.  Every block walks chunks of the concatenated list and
 // leaves one partial; the blocks of the second kernel each add all partials
 // in the same order, so the result does not depend on timing.
+// 290 arrays of 354 M elements, mostly float16: 366 us a call, of which the
+// first pass (708 MB) takes 124 us and the second (1416 MB, backwards, as what
+// was read last lies in L2) 222: 5.7 and 6.4 TB/s.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 

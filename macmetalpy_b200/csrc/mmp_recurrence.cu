@@ -25,9 +25,12 @@
 // next span before they replay the last and do not wait for it.
 // Every input is read once and every output written once; no block waits for
 // one outside its cluster, nothing is allocated, and the order of all
-// operations is fixed by the sizes.  What bounds it is HBM traffic, so the
-// loads run ahead: each thread copies the steps of its next spans with
-// cp.async into a ring in shared memory that only it reads.
+// operations is fixed by the sizes and the way rows are copied.  What bounds
+// it is HBM traffic, so the loads run ahead: each warp copies the rows of its
+// next spans into a ring in shared memory that only it reads.
+// Whole calls: 1 x 65521 x 1000 float32 121 to 131 us (6.0 to 6.5 TB/s); 8 x
+// 2048 x 2048 float16 gated 44 us (4.6 TB/s; latency, and 256 blocks on 148
+// SMs), its gradient 76 (5.3); 2 x 16383 x 1536 float32 gradient 176 (5.7).
 #include <cooperative_groups.h>
 #include <cuda.h>
 #include <cuda_fp16.h>
@@ -104,29 +107,21 @@ template <class V> __device__ __forceinline__ void rec_store(void *p, const V &v
 }
 
 template <int BYTES> __device__ __forceinline__ void rec_cp_async(unsigned dst, const void *src) {
-  if (BYTES == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
 }
 __device__ __forceinline__ void rec_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // Waits until at most `n` of this thread's newest groups are still on the way.
 __device__ __forceinline__ void rec_wait(int n) {
-  switch (n) {
-    case 0: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
-    case 1: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
-    case 2: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
-    case 3: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
-    case 4: asm volatile("cp.async.wait_group 4;" ::: "memory"); break;
-    default: asm volatile("cp.async.wait_group 5;" ::: "memory"); break;
-  }
+  if (n >= 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
+  else if (n == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
+  else asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 // The cluster's exchange: st.async writes into the other blocks' shared memory
 // and counts its bytes on a barrier there.  A fence in its place (the release
 // of barrier.cluster) waits for this block's own loads and stores on the way,
-// the ring's loads ahead among them: 314 us against 302 for 1 x 65521 x 1000
-// float32.
+// the ring's loads ahead among them (1 x 65521 x 1000 float32 with two stages
+// of 4-byte copies: 231 us against 216).
 __device__ __forceinline__ unsigned rec_map(const void *p, int rank) {
   unsigned r;
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"((unsigned)__cvta_generic_to_shared(p)), "r"(rank));
@@ -242,12 +237,6 @@ __global__ void __launch_bounds__(32 * (kRecWarps + 1), 2) rec_kernel(
     rank = (int)cg::this_cluster().block_rank();
     ranks = (int)cg::this_cluster().num_blocks();
     blk = blockIdx.x / ranks;
-    // every block of the cluster has to run, its barriers set up, before it is sent anything
-    if (w == 0 && lane < 2)
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"((unsigned)__cvta_generic_to_shared(&s_bar[lane]))
-                   : "memory");
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   }
   // the lane's chains: of a row of tiles for tensor copies, else of all groups in a row
   long long o, i;
@@ -277,12 +266,23 @@ __global__ void __launch_bounds__(32 * (kRecWarps + 1), 2) rec_kernel(
   chain_next();
   const int span = ranks * warps * N;  // steps of the cluster
   const int mine = (rank * warps + w) * N;
+  S carry[VEC];  // the joining warp's: the state before the cluster's present span
+#pragma unroll
+  for (int v = 0; v < VEC; ++v)
+    carry[v] = w == warps && active && g.seed ? ((const S *)g.seed)[chain + v] : S(0);
+  if (CLUSTER) {
+    // Every block of the cluster has to run, its barriers set up, before it is
+    // sent anything, and to have read the first state, whose place the last
+    // one may be written to.
+    if (w == 0 && lane < 2)
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"((unsigned)__cvta_generic_to_shared(&s_bar[lane]))
+                   : "memory");
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  }
   if (w == warps) {
     // The joining warp, beside the warps that compose and replay: a lane has
     // the chains of its group.
-    S carry[VEC];  // the state before the cluster's present span
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) carry[v] = active && g.seed ? ((const S *)g.seed)[chain + v] : S(0);
     if (CLUSTER) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     bool heard = true;
     for (int it = 0; it < g.iters; ++it) {
