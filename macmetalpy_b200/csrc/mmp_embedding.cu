@@ -847,7 +847,8 @@ int run_emb_grad(const void *ids_, int64_t n, const void *grad_, int64_t g_strid
   if (cluster) {
     const int items = (int)((n + mmpd::kSortThreads * mmpd::kSortRanks - 1) / (mmpd::kSortThreads * mmpd::kSortRanks));
     const int passes = (bits + mmpd::kSortBits - 1) / mmpd::kSortBits, digit = (bits + passes - 1) / passes;
-    // the sort takes some 10 us: as many zeros beside it as are written in that time
+    // the sort takes some 10 us: as many zeros beside it as are written in that
+    // time (16384 tokens, 50257 x 2048 float16: 69.7 us; with 24 MB 70.1, 48 MB 71.9)
     const int64_t row = width * (int64_t)sizeof(T), most = (int64_t)32 << 20;
     e.zeros = (unsigned)(rows * row < most ? rows : most / row);
     // one block an SM in clusters of eight, with 64 KB of zeros each at least
