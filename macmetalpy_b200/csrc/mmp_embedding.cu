@@ -899,7 +899,7 @@ int mmp_embedding(int dtype, const void *weight, int64_t rows, int64_t width, in
   if (rc) return rc;
   if (n == 0 || width == 0) return MMP_OK;
   if (!ids || !out || (rows && !weight)) return mmp::set_error(MMP_E_ARG, "embedding: null pointer");
-  if (!mmp::stream()) return mmp::set_error(MMP_E_CUDA, "no CUDA device available");
+  if (!mmp::device_error_word()) return mmp::set_error(MMP_E_CUDA, "no CUDA device available");
   MMP_EMB_DISPATCH(run_emb, weight, rows, width, w_stride, ids, n, scale, out);
 }
 
@@ -909,7 +909,7 @@ int mmp_embedding_grad(int dtype, int ids_dtype, const void *ids, int64_t n, con
   if (rc) return rc;
   if (rows == 0 || width == 0) return MMP_OK;
   if ((n && (!ids || !grad)) || !grad_weight) return mmp::set_error(MMP_E_ARG, "embedding_grad: null pointer");
-  if (!mmp::stream()) return mmp::set_error(MMP_E_CUDA, "no CUDA device available");
+  if (!mmp::device_error_word()) return mmp::set_error(MMP_E_CUDA, "no CUDA device available");
   MMP_EMB_DISPATCH(run_emb_grad, ids, n, grad, g_stride, rows, width, scale, padding_idx, grad_weight);
 }
 

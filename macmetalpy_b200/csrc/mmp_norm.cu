@@ -236,8 +236,8 @@ extern "C" int mmp_global_norm(int64_t count, const int *dtypes, const void *con
     if (sizes[i] < 0) return mmp::set_error(MMP_E_ARG, "global_norm: negative size");
     if (sizes[i] && (!x[i] || (y && !y[i]))) return mmp::set_error(MMP_E_ARG, "global_norm: null pointer");
   }
+  if (!mmp::device_error_word()) return mmp::set_error(MMP_E_CUDA, "no CUDA device available");
   cudaStream_t st = mmp::stream();
-  if (!st) return mmp::set_error(MMP_E_CUDA, "no CUDA device available");
   const int64_t most = (int64_t)mmp::sm_count() * 8;
   const int64_t launches = count ? (count + mmpd::kNormTable - 1) / mmpd::kNormTable : 1;
   double *partial = nullptr;

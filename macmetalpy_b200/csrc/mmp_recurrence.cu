@@ -895,7 +895,7 @@ int mmp_recurrence(int dtype, int gated, int64_t outer, int64_t steps, int64_t i
   const long long chains = outer * inner;
   if (chains == 0) return MMP_OK;
   if (steps > 0 && (!a || !x || !h)) return mmp::set_error(MMP_E_ARG, "recurrence: null pointer");
-  if (!mmp::stream()) return mmp::set_error(MMP_E_CUDA, "no CUDA device available");
+  if (!mmp::device_error_word()) return mmp::set_error(MMP_E_CUDA, "no CUDA device available");
   RecArgs g = {};
   g.in[0] = RecView{a, a_so, a_st};
   g.in[1] = RecView{x, x_so, x_st};
@@ -919,7 +919,7 @@ int mmp_recurrence_grad(int dtype, int gated, int64_t outer, int64_t steps, int6
   if (chains == 0) return MMP_OK;
   if (steps > 0 && (!a || (gated && !x) || !h || !grad || !grad_a || !grad_x))
     return mmp::set_error(MMP_E_ARG, "recurrence_grad: null pointer");
-  if (!mmp::stream()) return mmp::set_error(MMP_E_CUDA, "no CUDA device available");
+  if (!mmp::device_error_word()) return mmp::set_error(MMP_E_CUDA, "no CUDA device available");
   RecArgs r = {};
   r.in[0] = RecView{a, a_so, a_st};
   r.in[1] = RecView{grad, g_so, g_st};

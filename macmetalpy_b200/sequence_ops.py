@@ -249,8 +249,9 @@ def linear_recurrence_grad(a, x, h, grad, h0=None, *, axis=-2, gated=False, grad
     one with respect to the state after the last step, for a sequence that went
     on in another call.  With ``gated=False``, ``x`` is not read and may be None.
 
-    Returns ``(grad_a, grad_x, grad_h0)``: the first two in the arrays' dtype,
-    the last in the state's dtype, or None where ``h0`` is None.  ``out``, a
+    Returns ``(grad_a, grad_x, grad_h0)``: the first two in the arrays' shape and
+    dtype (for a broadcast view, sum them over its broadcast axes), the last in
+    the state's dtype, or None where ``h0`` is None.  ``out``, a
     tuple of two or three arrays, receives them (the first two may be ``a``,
     ``x`` or ``grad`` themselves, not one another).
     """
