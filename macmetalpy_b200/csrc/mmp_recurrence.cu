@@ -21,8 +21,8 @@
 //            other's shared memory; then the cluster moves on along the axis
 // A span's steps run twice, once to compose it and once, from the state then
 // known, for the outputs.  One more warp of the block joins the spans; where
-// the gates need not stay in registers in between, the others compose the
-// next span before they replay the last and do not wait for it.
+// the gates do not stay in registers in between (HOLD), the others compose
+// the next span before they replay the last and do not wait for it.
 // Every input is read once and every output written once; no block waits for
 // one outside its cluster, nothing is allocated, and the order of all
 // operations is fixed by the sizes and the way rows are copied.  What bounds
@@ -212,7 +212,10 @@ __device__ __forceinline__ void rec_tma(unsigned dst, const RecMap3 &map, unsign
       : "memory");
 }
 
-template <class T, int VEC, int COPY, bool GRAD, bool GATED, bool CLUSTER>
+// HOLD: gates of a span stay in registers from compose to replay, which then
+// follow one another; else they are evaluated twice, and a span is composed
+// while the one before it is joined.
+template <class T, int VEC, int COPY, bool GRAD, bool GATED, bool CLUSTER, bool HOLD>
 __global__ void __launch_bounds__(32 * (kRecWarps + 1), 2) rec_kernel(
     const __grid_constant__ RecArgs g, const __grid_constant__ RecMaps<COPY> maps) {
   typedef typename RecState<T>::type S;
@@ -224,8 +227,7 @@ __global__ void __launch_bounds__(32 * (kRecWarps + 1), 2) rec_kernel(
   constexpr bool ASYNC = COPY == kLane;
   constexpr int kStages = 3;
   extern __shared__ __align__(128) unsigned char s_ring[];
-  constexpr bool HOLD = GATED && !CLUSTER;  // gates of a span stay in registers from compose to replay
-  constexpr int LAG = HOLD ? 0 : 1;         // spans between compose and replay
+  constexpr int LAG = HOLD ? 0 : 1;  // spans between compose and replay
   __shared__ __align__(16) RecMap<S> s_map[2][kRecWarps][NC];                      // the warps' spans
   __shared__ __align__(16) RecMap<S> s_blk[CLUSTER ? 2 : 1][CLUSTER ? 8 : 1][NC];  // the cluster's blocks' spans
   __shared__ __align__(16) S s_start[2][kRecWarps][NC];                            // states before the warps' spans
@@ -722,9 +724,9 @@ int rec_sizes(const char *what, int dtype, int64_t outer, int64_t steps, int64_t
   return MMP_OK;
 }
 
-template <class T, int VEC, int COPY, bool GRAD, bool GATED, bool CLUSTER>
+template <class T, int VEC, int COPY, bool GRAD, bool GATED, bool CLUSTER, bool HOLD>
 int rec_launch(const RecArgs &g, const mmpd::RecMaps<COPY> &maps, unsigned blocks, int ranks, size_t smem) {
-  auto fn = mmpd::rec_kernel<T, VEC, COPY, GRAD, GATED, CLUSTER>;
+  auto fn = mmpd::rec_kernel<T, VEC, COPY, GRAD, GATED, CLUSTER, HOLD>;
   if (smem > 16 * 1024)  // together with the static part this can pass the default 48 KB
     MMP_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   // the composing warps and the joining one
@@ -818,8 +820,17 @@ int rec_run(RecArgs g) {
       if (rc) return rc;
     }
   }
-  return ranks > 1 ? rec_launch<T, VEC, COPY, GRAD, GATED, true>(g, maps, (unsigned)blocks, ranks, smem)
-                   : rec_launch<T, VEC, COPY, GRAD, GATED, false>(g, maps, (unsigned)blocks, ranks, smem);
+  // Gates are held where blocks stand alone (8 x 2048 x 2048 float16 44 us,
+  // evaluated twice 63).  In clusters that leaves the exchange uncovered: it
+  // pays forward and for float64 where SMs have two blocks (1 x 16384 x 2048
+  // float16 58 us against 66, its gradient 107 against 93; 1 x 65536 x 512, 64
+  // blocks, 154 against 134; 1 x 8192 x 1024 float64 57 against 75, its gradient
+  // 87 against 96).
+  constexpr bool can_hold = GATED && (!GRAD || sizeof(T) == 8);
+  if (ranks == 1) return rec_launch<T, VEC, COPY, GRAD, GATED, false, GATED>(g, maps, (unsigned)blocks, 1, smem);
+  if constexpr (can_hold)
+    if (blocks * ranks > sms) return rec_launch<T, VEC, COPY, GRAD, GATED, true, true>(g, maps, (unsigned)blocks, ranks, smem);
+  return rec_launch<T, VEC, COPY, GRAD, GATED, true, false>(g, maps, (unsigned)blocks, ranks, smem);
 }
 
 // Whether every operand can be moved in pieces of `bytes` (e: element size).

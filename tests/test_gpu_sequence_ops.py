@@ -228,6 +228,31 @@ def test_recurrence_long(cp, dt, gated, shape):
     close(got[2].get(), dh0, e0 * UNIT[dt], str(h0.dtype))
 
 
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("shape", [(3, 701, 257), (6, 640, 258), (2, 1000, 512)])
+def test_recurrence_gated_in_clusters(cp, dt, shape):
+    """25 to 32 blocks of chains, in clusters of eight, for each way rows are
+    copied; gates that keep and that replace the state; equal calls give equal
+    bits."""
+    a, x, h0, g, gs = rec_inputs(shape, dt, True, 700)
+    a[:, 350], a[:, 353] = np.inf, -np.inf
+    hs, es, last, el = recurrence(a, x, h0, True)
+    sdt = "float64" if dt == "float64" else "float32"
+    state = cp.empty((shape[0], shape[2]), dtype=sdt)
+    h = cp.linear_recurrence(cp.array(a), cp.array(x), cp.array(h0), gated=True, state_out=state)
+    close(h.get(), hs, es * UNIT[dt], dt)
+    close(state.get(), last, el * UNIT[dt], sdt)
+    again = cp.linear_recurrence(cp.array(a), cp.array(x), cp.array(h0), gated=True)
+    np.testing.assert_array_equal(again.get(), h.get())
+    h = hs.astype(dt)
+    da, dx, dh0, ea, ex, e0 = recurrence_grad(a, x, h, g, h0, gs, True)
+    got = cp.linear_recurrence_grad(cp.array(a), cp.array(x), cp.array(h), cp.array(g), cp.array(h0), gated=True,
+                                    grad_state=cp.array(gs))
+    close(got[0].get(), da, ea * UNIT[dt], dt)
+    close(got[1].get(), dx, ex * UNIT[dt], dt)
+    close(got[2].get(), dh0, e0 * UNIT[dt], sdt)
+
+
 def test_recurrence_decays_above_one(cp):
     """Spans whose decays multiply past float32's range: a state of zero stays
     zero, and what is finite step by step is finite."""
