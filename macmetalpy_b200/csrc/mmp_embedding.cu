@@ -28,6 +28,7 @@
 #include <cuda_runtime.h>
 
 #include <type_traits>
+#include <utility>
 
 #include "mmp_chain.cuh"
 #include "mmp_device.cuh"
@@ -323,6 +324,9 @@ __global__ void __cluster_dims__(kSortRanks, 1, 1) __launch_bounds__(kSortThread
   }
   EmbSortSmem &s = *reinterpret_cast<EmbSortSmem *>(s_raw);
   cg::cluster_group cl = cg::this_cluster();
+  // No block may reach into another's shared memory before that one runs:
+  // what the first pass sends waits for this barrier, the ids' loads do not.
+  auto running = cl.barrier_arrive();
   const unsigned rank = cl.block_rank();
   const unsigned tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const unsigned tile = items * kSortThreads;
@@ -346,6 +350,7 @@ __global__ void __cluster_dims__(kSortRanks, 1, 1) __launch_bounds__(kSortThread
       buf[0][p] = (unsigned long long)(ok && id[e] != padding ? id[e] : rows) << 32 | i;
     }
   }
+  cl.barrier_wait(std::move(running));
   for (int pass = 0; pass < passes; ++pass) {
     const int shift = 32 + pass * digit;
     const unsigned mask = (1u << digit) - 1;
