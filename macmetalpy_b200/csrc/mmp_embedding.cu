@@ -32,6 +32,7 @@
 
 #include "mmp_chain.cuh"
 #include "mmp_device.cuh"
+#include "mmp_embedding_plan.h"
 #include "mmp_internal.h"
 
 namespace mmpd {
@@ -155,7 +156,9 @@ constexpr unsigned kEmbFew = 1024;       // tokens up to which no sort is made
 constexpr unsigned kEmbFewBits = 16384;  // rows a block of that path marks at once
 
 // Zeros of the rows [r0, rows) whose bit in `seen` is not set, by warps
-// `warp`, `warp` + `warps`, ..., `unit` rows of a word at a time.
+// `warp`, `warp` + `warps`, ..., `unit` rows of a word at a time: r0 is a
+// multiple of `unit`, a power of two up to 32, so that no unit reaches into
+// the next word (EmbZeroPlan).
 template <class T>
 __device__ __forceinline__ void emb_zero_marked(const unsigned *__restrict__ seen, unsigned r0, unsigned rows,
                                                 unsigned width, T *__restrict__ out, unsigned unit, unsigned warp,
@@ -785,7 +788,8 @@ struct EmbSorted {
   unsigned *keys, *order, *runs, *seen;
   mmpd::EmbRun *list;
   void *part;
-  unsigned n, zeros;  // rows below `zeros` have theirs
+  unsigned n;
+  mmp::EmbZeroPlan zeros;
   EmbShares sh;
 };
 
@@ -794,21 +798,16 @@ int emb_sum(const EmbSorted &e, const T *grad, int64_t g_stride, int64_t rows, i
   typedef typename mmpd::EmbAcc<T>::type S;
   const unsigned n = e.n, lanes = e.sh.lanes, slices = e.sh.slices, groups = e.sh.groups, share = e.sh.share,
                  shares = e.sh.shares;
-  // Beside them two blocks an SM that write zeros, 8 KB of rows a warp at a
-  // time; the last 24 MB are left for the joining kernel, which waits for
-  // memory some 6 us and moves next to nothing.
-  const int64_t row = width * (int64_t)sizeof(T), late = ((int64_t)24 << 20) / row;
-  const unsigned zeros_end = (unsigned)(rows - e.zeros > 2 * late ? (rows - late) / 32 * 32 : rows);
-  unsigned unit = 32;
-  while (unit > 1 && unit * row > 8192) unit /= 2;
+  // beside them two blocks an SM that write zeros
+  const unsigned zeros = e.zeros.first, zeros_end = e.zeros.second, unit = e.zeros.unit;
   auto zero_grid = [&](unsigned from, unsigned to, unsigned most) {
     const uint64_t want = ((uint64_t)(to - from + unit - 1) / unit + 7) / 8;
     return (unsigned)(want < most ? want : most);
   };
-  const unsigned zero_blocks = zero_grid(e.zeros, zeros_end, 2 * (unsigned)mmp::sm_count());
+  const unsigned zero_blocks = zero_grid(zeros, zeros_end, 2 * (unsigned)mmp::sm_count());
   const int rc = mmp::launch_after(mmpd::emb_sum_kernel<T, VEC>, dim3(zero_blocks + (shares + groups - 1) / groups, slices), 256, 0, 1, e.keys,
                         e.order, n, share, shares, lanes, grad, g_stride, (unsigned)rows, (unsigned)width, (S)scale, out,
-                        (S *)e.part, e.runs, e.list, e.seen, e.zeros, zeros_end, unit, zero_blocks);
+                        (S *)e.part, e.runs, e.list, e.seen, zeros, zeros_end, unit, zero_blocks);
   if (rc) return rc;
   constexpr int JV = VEC >= 4 ? 4 : 1;
   const unsigned cols = (unsigned)((width + 32 * JV - 1) / (32 * JV));
@@ -838,6 +837,7 @@ int run_emb_grad(const void *ids_, int64_t n, const void *grad_, int64_t g_strid
   e.sh = emb_shares(e.n, width, vec);
   // keys, order (a second time each for sort_pairs), parts, list, bitmap, count
   const bool cluster = n <= mmpd::kEmbCluster;
+  e.zeros = mmp::emb_zero_plan(rows, width * (int64_t)sizeof(T), cluster);
   const size_t np = ((size_t)n + 7) & ~(size_t)7, words = ((size_t)rows + 31) / 32;
   const size_t parts = (size_t)e.sh.shares * 2 * width * sizeof(typename mmpd::EmbAcc<T>::type);
   const size_t sorted = np * (cluster ? 8 : 16), lists = ((size_t)e.sh.shares * sizeof(mmpd::EmbRun) + 15) / 16 * 16;
@@ -852,27 +852,23 @@ int run_emb_grad(const void *ids_, int64_t n, const void *grad_, int64_t g_strid
   if (cluster) {
     const int items = (int)((n + mmpd::kSortThreads * mmpd::kSortRanks - 1) / (mmpd::kSortThreads * mmpd::kSortRanks));
     const int passes = (bits + mmpd::kSortBits - 1) / mmpd::kSortBits, digit = (bits + passes - 1) / passes;
-    // the sort takes some 10 us: as many zeros beside it as are written in that
-    // time (16384 tokens, 50257 x 2048 float16: 69.7 us; with 24 MB 70.1, 48 MB 71.9)
-    const int64_t row = width * (int64_t)sizeof(T), most = (int64_t)32 << 20;
-    e.zeros = (unsigned)(rows * row < most ? rows : most / row);
+    const int64_t zeros = e.zeros.first, row = width * (int64_t)sizeof(T);
     // one block an SM in clusters of eight, with 64 KB of zeros each at least
     const int64_t all = mmp::sm_count() / mmpd::kSortRanks - 1;
-    const int64_t want = (int64_t)e.zeros * row / (65536 * mmpd::kSortRanks) + 1;
+    const int64_t want = zeros * row / (65536 * mmpd::kSortRanks) + 1;
     const unsigned clusters = 1 + (unsigned)(want < all ? want : all);
-    const int64_t share = ((int64_t)e.zeros + (clusters - 1) * mmpd::kSortRanks - 1) / ((clusters - 1) * mmpd::kSortRanks);
+    const int64_t share = (zeros + (clusters - 1) * mmpd::kSortRanks - 1) / ((clusters - 1) * mmpd::kSortRanks);
     size_t smem = sizeof(mmpd::EmbSortSmem) + (size_t)items * mmpd::kSortThreads * 16;
     const size_t seen = (size_t)(share < 524288 ? (share + 31) / 32 * 4 : 65536);
     if (smem < seen) smem = seen;
     auto fn = mmpd::emb_sort_kernel<T, I>;
     MMP_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     rc = mmp::launch_after(fn, dim3(clusters * mmpd::kSortRanks), mmpd::kSortThreads, smem, 1, ids, (unsigned)n, rows, padding,
-                          items, passes, digit, e.keys, e.order, (unsigned)width, out, e.zeros, (unsigned)(seen * 8),
+                          items, passes, digit, e.keys, e.order, (unsigned)width, out, (unsigned)zeros, (unsigned)(seen * 8),
                           e.seen, e.runs, err);
     if (rc) return rc;
   } else {
     unsigned *const kb[2] = {e.keys, e.keys + 2 * np}, *const ob[2] = {e.order, e.order + 2 * np};
-    e.zeros = 0;
     MMP_CUDA_TRY(cudaMemsetAsync(e.seen, 0, words * 4 + 4, mmp::stream()));
     mmpd::emb_prep_kernel<I><<<mmp::sm_count() * 2, 256, 0, mmp::stream()>>>(ids, (unsigned)n, rows, padding, kb[0],
                                                                              ob[0], e.seen, err);
