@@ -62,3 +62,56 @@ def test_embedding_grad_large_tables(cp, rows, width, dt, kind):
         ids = np.resize(np.arange(0, rows, 32), n) if rows <= 32 * n else ids // 32 * 32
     g = rng.standard_normal((n, width), dtype=np.float32).astype(dt)
     check_table_grad(cp, ids, g, rows, calls=3)
+
+
+@pytest.mark.parametrize("idt", ["int32", "int64"])
+@pytest.mark.parametrize("dt", ["float16", "float32", "float64"])
+def test_embedding_grad_more_tokens_than_a_cluster_sorts(cp, dt, idt):
+    """65536 tokens (the cluster's last), one more, and ordinary batches: tables
+    of one row to a million, frequent ids, padding, equal bits of equal calls."""
+    for i, (n, rows, width) in enumerate([(65536, 5000, 24), (65537, 5000, 24), (65543, 1, 3), (131072, 50257, 16),
+                                          (70001, 1000003, 9), (200003, 300, 40), (100000, 1 << 18, 4)]):
+        rng = np.random.default_rng(i)
+        ids = np.minimum(np.exp(rng.random(n) * np.log(rows + 1)) - 1, rows - 1).astype(idt)
+        g = rng.standard_normal((n, width), dtype=np.float32).astype(dt)
+        want, err = table_grad(ids, g, rows, 0.3)
+        pad = int(ids[5]) if i % 2 else None
+        if pad is not None:
+            want[pad] = 0
+        I, G = cp.array(ids), cp.array(g)
+        got = cp.embedding_grad(I, G, rows, 0.3, padding_idx=pad, out=cp.full((rows, width), 5, dtype=dt)).get()
+        close(got, want, err * UNIT[dt], dt)
+        if pad is not None:
+            assert not got[pad].any()
+        np.testing.assert_array_equal(cp.embedding_grad(I, G, rows, 0.3, padding_idx=pad).get(), got)
+    cp.synchronize()
+
+
+@pytest.mark.parametrize("kind", ["one", "two", "all", "bad"])
+def test_embedding_grad_many_tokens_of_a_kind(cp, kind):
+    """One id, two in turn, each once, and ids out of range among others (which
+    add nothing and are reported)."""
+    n, rows, width = 90001, 120000, 20
+    rng = np.random.default_rng(4)
+    ids = {"one": np.full(n, 77), "two": np.arange(n) % 2 * (rows - 1), "all": rng.permutation(rows)[:n],
+           "bad": rng.integers(0, rows, n)}[kind]
+    g = rng.standard_normal((n, width), dtype=np.float32)
+    sent, keep = ids.copy(), np.ones(n, bool)
+    if kind == "bad":
+        keep = rng.random(n) < 0.9
+        sent[~keep] = np.resize([-1, rows, 2 ** 40], int((~keep).sum()))
+    want, err = table_grad(ids[keep], g[keep], rows, 1.0)
+    got = cp.embedding_grad(cp.array(sent), cp.array(g), rows).get()
+    close(got, want, err * UNIT["float32"], "float32")
+    if kind == "bad":
+        with pytest.raises(RuntimeError, match="5"):
+            cp.synchronize()
+    cp.synchronize()
+
+
+def test_embedding_grad_many_tokens_large_table(cp):
+    rng = np.random.default_rng(2)
+    check_table_grad(cp, rng.integers(0, 50257, 131072), rng.standard_normal((131072, 100), dtype=np.float32)
+                     .astype(np.float16), 50257)
+    check_table_grad(cp, np.resize(np.arange(0, 400009, 32), 70000), rng.standard_normal((70000, 50), dtype=np.float32),
+                     400009)
