@@ -2,7 +2,8 @@
 // launch_after may be set up while the one before it in the stream ends.  It
 // calls chain_wait before it touches memory, which waits until that one is
 // done and its writes are there, and chain_next to let the one behind it be
-// set up in turn.
+// set up in turn.  Its inputs are no `const __restrict__`, which would promise
+// the compiler that nothing writes them while the kernel runs.
 #pragma once
 #include <cuda_runtime.h>
 

@@ -19,7 +19,10 @@
 //                several shares are joined.  The zeros are written beside the
 //                sort and beside the sums: writes alone reach 3.9 TB/s here
 //                (a plain fill), with reads next to them 6.5 in all.
-// No float is added atomically, so equal calls give equal bits.
+// No float is added atomically, so equal calls give equal bits.  Inputs are
+// not marked __restrict__: a kernel launched by launch_after is resident while
+// the one before it still writes them, and a load that passes for one of
+// constant memory need not stay behind chain_wait.
 // Whole calls: lookup of 16384 x 1024 float32 18 us (writes alone take 17 at
 // the fill rate); gradient of 512 tokens, 8192 x 768 float32 10 us, of 16384
 // tokens, 50257 x 2048 float16 70 us (fill rate 52, copy rate 42).
@@ -46,8 +49,8 @@ template <class T, int VEC> struct alignas(sizeof(T) * VEC) EmbVec { T v[VEC]; }
 
 // ---- lookup: a thread moves U vectors; vectors of a row are neighbours.
 template <class T, class I, int VEC, int U>
-__global__ void __launch_bounds__(256) emb_kernel(const T *__restrict__ w, long long rows, FastDiv per,
-                                                  long long w_stride, const I *__restrict__ ids, unsigned total,
+__global__ void __launch_bounds__(256) emb_kernel(const T *w, long long rows, FastDiv per,
+                                                  long long w_stride, const I *ids, unsigned total,
                                                   typename EmbAcc<T>::type scale, T *__restrict__ out, int *err) {
   typedef typename EmbAcc<T>::type S;
   typedef EmbVec<T, VEC> V;
@@ -64,11 +67,11 @@ __global__ void __launch_bounds__(256) emb_kernel(const T *__restrict__ w, long 
     id[u] = i < total ? (long long)ids[r] : -1;
   }
   V v[U];
+  bool bad = false;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const unsigned i = i0 + u * 256u;
     const bool ok = id[u] >= 0 && id[u] < rows;
-    if (i < total && !ok) atomicExch(err, 5);
+    bad |= !ok && i0 + u * 256u < total;
     if (ok) {
       v[u] = *reinterpret_cast<const V *>(w + id[u] * w_stride + (long long)col[u] * VEC);
     } else {
@@ -84,6 +87,7 @@ __global__ void __launch_bounds__(256) emb_kernel(const T *__restrict__ w, long 
     for (int e = 0; e < VEC; ++e) v[u].v[e] = Cvt<T, S>::f(Cvt<S, T>::f(v[u].v[e]) * scale);
     *reinterpret_cast<V *>(out + (long long)i * VEC) = v[u];
   }
+  if (bad) atomicExch(err, 5);
 }
 
 // Zeros to `n` elements by one warp: 16-byte pieces, the ends element by
@@ -108,7 +112,7 @@ template <class T> __device__ __forceinline__ void emb_zero(T *p, long long n) {
 // bitmap of at least r1 - r0 bits.  A warp takes `unit` rows of one word of
 // it; neighbouring rows without a token are one stretch of memory.
 template <class T, class I>
-__device__ void emb_zero_rows(const I *__restrict__ ids, unsigned n, long long rows, long long padding, long long r0,
+__device__ void emb_zero_rows(const I *ids, unsigned n, long long rows, long long padding, long long r0,
                               long long r1, unsigned width, T *__restrict__ out, unsigned *s_seen, int *err) {
   const unsigned tid = threadIdx.x, nt = blockDim.x;
   const unsigned count = (unsigned)(r1 - r0);
@@ -160,7 +164,7 @@ constexpr unsigned kEmbFewBits = 16384;  // rows a block of that path marks at o
 // multiple of `unit`, a power of two up to 32, so that no unit reaches into
 // the next word (EmbZeroPlan).
 template <class T>
-__device__ __forceinline__ void emb_zero_marked(const unsigned *__restrict__ seen, unsigned r0, unsigned rows,
+__device__ __forceinline__ void emb_zero_marked(const unsigned *seen, unsigned r0, unsigned rows,
                                                 unsigned width, T *__restrict__ out, unsigned unit, unsigned warp,
                                                 unsigned warps) {
   for (unsigned long long r = r0 + (unsigned long long)warp * unit; r < rows; r += (unsigned long long)warps * unit) {
@@ -189,7 +193,7 @@ __device__ __forceinline__ void emb_mark(unsigned *seen, unsigned id, bool want)
 // ---- few tokens, one launch.  Blocks [0, n): token blockIdx.x, if it is the
 // first of its id, adds all of them in the order of n.  The others: zeros.
 template <class T, class I, int VEC>
-__global__ void __launch_bounds__(256) emb_grad_few(const I *__restrict__ ids, unsigned n, const T *__restrict__ grad,
+__global__ void __launch_bounds__(256) emb_grad_few(const I *ids, unsigned n, const T *grad,
                                                     long long g_stride, long long rows, unsigned width,
                                                     typename EmbAcc<T>::type scale, long long padding,
                                                     T *__restrict__ out, int *err) {
@@ -313,7 +317,7 @@ __device__ __forceinline__ unsigned emb_scan_bins(unsigned v, unsigned *s_sum) {
 // `seen`.  The other clusters write the zeros of the rows below `zeros`.
 template <class T, class I>
 __global__ void __cluster_dims__(kSortRanks, 1, 1) __launch_bounds__(kSortThreads, 1)
-    emb_sort_kernel(const I *__restrict__ ids, unsigned n, long long rows, long long padding, int items, int passes,
+    emb_sort_kernel(const I *ids, unsigned n, long long rows, long long padding, int items, int passes,
                     int digit, unsigned *__restrict__ keys, unsigned *__restrict__ order, unsigned width,
                     T *__restrict__ out, unsigned zeros, unsigned bits, unsigned *__restrict__ seen,
                     unsigned *__restrict__ runs, int *err) {
@@ -453,7 +457,7 @@ __global__ void __cluster_dims__(kSortRanks, 1, 1) __launch_bounds__(kSortThread
 
 // ---- more tokens than a cluster holds: keys for sort_pairs, and the marks.
 template <class I>
-__global__ void __launch_bounds__(256) emb_prep_kernel(const I *__restrict__ ids, unsigned n, long long rows,
+__global__ void __launch_bounds__(256) emb_prep_kernel(const I *ids, unsigned n, long long rows,
                                                        long long padding, unsigned *__restrict__ keys,
                                                        unsigned *__restrict__ order, unsigned *__restrict__ seen,
                                                        int *err) {
@@ -481,14 +485,14 @@ struct EmbRun {
 };
 
 template <class T, int VEC>
-__global__ void __launch_bounds__(256) emb_sum_kernel(const unsigned *__restrict__ keys,
-                                                      const unsigned *__restrict__ order, unsigned n, unsigned share,
-                                                      unsigned shares, unsigned lanes, const T *__restrict__ grad,
+__global__ void __launch_bounds__(256) emb_sum_kernel(const unsigned *keys,
+                                                      const unsigned *order, unsigned n, unsigned share,
+                                                      unsigned shares, unsigned lanes, const T *grad,
                                                       long long g_stride, unsigned rows, unsigned width,
                                                       typename EmbAcc<T>::type scale, T *__restrict__ out,
                                                       typename EmbAcc<T>::type *__restrict__ part,
                                                       unsigned *__restrict__ runs, EmbRun *__restrict__ list,
-                                                      const unsigned *__restrict__ seen, unsigned zeros,
+                                                      const unsigned *seen, unsigned zeros,
                                                       unsigned zeros_end, unsigned unit, unsigned zero_blocks) {
   typedef typename EmbAcc<T>::type S;
   typedef EmbVec<T, VEC> V;
@@ -615,10 +619,10 @@ __global__ void __launch_bounds__(256) emb_sum_kernel(const unsigned *__restrict
 // warps' sums in order.
 template <class T, int JV>
 __global__ void __launch_bounds__(256) emb_join_kernel(unsigned width, typename EmbAcc<T>::type scale,
-                                                       const typename EmbAcc<T>::type *__restrict__ part,
-                                                       const unsigned *__restrict__ runs,
-                                                       const EmbRun *__restrict__ list, T *__restrict__ out,
-                                                       const unsigned *__restrict__ seen, unsigned zeros, unsigned rows,
+                                                       const typename EmbAcc<T>::type *part,
+                                                       const unsigned *runs,
+                                                       const EmbRun *list, T *__restrict__ out,
+                                                       const unsigned *seen, unsigned zeros, unsigned rows,
                                                        unsigned unit, unsigned join_blocks) {
   typedef typename EmbAcc<T>::type S;
   typedef EmbVec<S, JV> V;

@@ -67,3 +67,20 @@ def test_shared_memory_of_other_blocks_after_a_cluster_barrier(kernel):
     to run: a barrier of the whole cluster comes before the first access."""
     body = ALL[kernel][1]
     assert cluster_sync(body) < re.search(SENDS, body).start()
+
+
+CHAINED = [p for p in SOURCES if "chain_wait();" in open(p).read()]
+
+
+@pytest.mark.parametrize("path", CHAINED, ids=os.path.basename)
+def test_chained_kernels_promise_nothing_of_their_inputs(path):
+    """A kernel that is set up while its predecessor still writes must not tell
+    the compiler that its inputs stay as they are: loads marked so (const
+    __restrict__, __ldg, ld.global.nc) need not stay behind the wait."""
+    text = re.sub(r"//[^\n]*", "", open(path).read())
+    assert not re.findall(r"const\s+[\w:<>, ]+\*\s*__restrict__[^,)]*", text)
+    assert "__ldg" not in text and "ld.global.nc" not in text
+
+
+def test_files_of_chained_kernels_are_found():
+    assert {"mmp_embedding.cu", "mmp_norm.cu", "mmp_recurrence.cu"} <= {os.path.basename(p) for p in CHAINED}
