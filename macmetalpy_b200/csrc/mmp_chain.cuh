@@ -7,6 +7,8 @@
 #pragma once
 #include <cuda_runtime.h>
 
+#include <atomic>
+
 #include "mmp_internal.h"
 
 namespace mmpd {
@@ -37,5 +39,23 @@ int launch_after(void (*fn)(P...), dim3 grid, dim3 block, size_t smem, int ranks
   MMP_CUDA_TRY(cudaLaunchKernelEx(&cfg, fn, P(args)...));
   return MMP_OK;
 }
+
+// A kernel's limit of dynamic shared memory, raised once per device to the most
+// that any of its launches asks for.  (A limit set to each call's own size
+// could be lowered by another thread between that and the launch.)  One
+// object per kernel.
+struct SmemLimit {
+  std::atomic<bool> set[64];
+  template <class... P>
+  int raise(void (*fn)(P...), size_t most) {
+    const int dev = current_device();
+    if (dev < 0 || dev >= 64) return set_error(MMP_E_ARG, "device out of range");
+    if (!set[dev].load(std::memory_order_acquire)) {
+      MMP_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
+      set[dev].store(true, std::memory_order_release);
+    }
+    return MMP_OK;
+  }
+};
 
 }  // namespace mmp

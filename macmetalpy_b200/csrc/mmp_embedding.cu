@@ -862,11 +862,15 @@ int run_emb_grad(const void *ids_, int64_t n, const void *grad_, int64_t g_strid
     const int64_t want = zeros * row / (65536 * mmpd::kSortRanks) + 1;
     const unsigned clusters = 1 + (unsigned)(want < all ? want : all);
     const int64_t share = (zeros + (clusters - 1) * mmpd::kSortRanks - 1) / ((clusters - 1) * mmpd::kSortRanks);
-    size_t smem = sizeof(mmpd::EmbSortSmem) + (size_t)items * mmpd::kSortThreads * 16;
-    const size_t seen = (size_t)(share < 524288 ? (share + 31) / 32 * 4 : 65536);
-    if (smem < seen) smem = seen;
+    auto bytes = [](int items) { return sizeof(mmpd::EmbSortSmem) + (size_t)items * mmpd::kSortThreads * 16; };
+    constexpr size_t kSeen = 65536;  // of bitmap a block at most
+    const size_t seen = share < (int64_t)kSeen * 8 ? (size_t)(share + 31) / 32 * 4 : kSeen;
+    const size_t smem = bytes(items) < seen ? seen : bytes(items);
     auto fn = mmpd::emb_sort_kernel<T, I>;
-    MMP_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    static mmp::SmemLimit limit;
+    static_assert(sizeof(mmpd::EmbSortSmem) + mmpd::kSortItems * mmpd::kSortThreads * 16 >= kSeen, "the limit");
+    rc = limit.raise(fn, bytes(mmpd::kSortItems));
+    if (rc) return rc;
     rc = mmp::launch_after(fn, dim3(clusters * mmpd::kSortRanks), mmpd::kSortThreads, smem, 1, ids, (unsigned)n, rows, padding,
                           items, passes, digit, e.keys, e.order, (unsigned)width, out, (unsigned)zeros, (unsigned)(seen * 8),
                           e.seen, e.runs, err);

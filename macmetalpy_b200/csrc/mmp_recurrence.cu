@@ -724,11 +724,20 @@ int rec_sizes(const char *what, int dtype, int64_t outer, int64_t steps, int64_t
   return MMP_OK;
 }
 
+// Bytes of the ring of `warps` warps.
+template <class T, int VEC, int COPY, bool GRAD, bool GATED> constexpr size_t rec_ring(int stages, int warps) {
+  constexpr int N = mmpd::RecSpan<(int)sizeof(T) * VEC, COPY, GRAD>::value, NA = GRAD ? (GATED ? 4 : 3) : 2;
+  return 128 + (size_t)stages * NA * N * warps * 32 * sizeof(T) * VEC;
+}
+template <int COPY> constexpr int kRecStages = COPY != mmpd::kPlain ? 3 : 2;  // at most
+
 template <class T, int VEC, int COPY, bool GRAD, bool GATED, bool CLUSTER, bool HOLD>
-int rec_launch(const RecArgs &g, const mmpd::RecMaps<COPY> &maps, unsigned blocks, int ranks, size_t smem) {
+int rec_launch(const RecArgs &g, const mmpd::RecMaps<COPY> &maps, unsigned blocks, int ranks) {
   auto fn = mmpd::rec_kernel<T, VEC, COPY, GRAD, GATED, CLUSTER, HOLD>;
-  if (smem > 16 * 1024)  // together with the static part this can pass the default 48 KB
-    MMP_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  static mmp::SmemLimit limit;
+  const int rc = limit.raise(fn, rec_ring<T, VEC, COPY, GRAD, GATED>(kRecStages<COPY>, mmpd::kRecWarps));
+  if (rc) return rc;
+  const size_t smem = rec_ring<T, VEC, COPY, GRAD, GATED>(g.stages, g.warps);
   // the composing warps and the joining one
   return mmp::launch_after(fn, blocks * ranks, dim3(32, g.warps + 1), smem, ranks, g, maps);
 }
@@ -810,9 +819,7 @@ int rec_run(RecArgs g) {
   if (blocks * ranks > INT32_MAX) return mmp::set_error(MMP_E_ARG, "recurrence: too many chains");
   g.iters = (int)((spans + (long long)warps * ranks - 1) / ((long long)warps * ranks));
   g.warps = warps;
-  const int most = COPY != mmpd::kPlain ? 3 : 2;
-  g.stages = g.iters < most ? g.iters : most;
-  const size_t smem = 128 + (size_t)g.stages * NA * N * warps * 32 * sizeof(T) * VEC;
+  g.stages = g.iters < kRecStages<COPY> ? g.iters : kRecStages<COPY>;
   mmpd::RecMaps<COPY> maps;
   if constexpr (COPY == mmpd::kTma) {
     for (int q = 0; q < NA; ++q) {
@@ -827,10 +834,10 @@ int rec_run(RecArgs g) {
   // blocks, 154 against 134; 1 x 8192 x 1024 float64 57 against 75, its gradient
   // 87 against 96).
   constexpr bool can_hold = GATED && (!GRAD || sizeof(T) == 8);
-  if (ranks == 1) return rec_launch<T, VEC, COPY, GRAD, GATED, false, GATED>(g, maps, (unsigned)blocks, 1, smem);
+  if (ranks == 1) return rec_launch<T, VEC, COPY, GRAD, GATED, false, GATED>(g, maps, (unsigned)blocks, 1);
   if constexpr (can_hold)
-    if (blocks * ranks > sms) return rec_launch<T, VEC, COPY, GRAD, GATED, true, true>(g, maps, (unsigned)blocks, ranks, smem);
-  return rec_launch<T, VEC, COPY, GRAD, GATED, true, false>(g, maps, (unsigned)blocks, ranks, smem);
+    if (blocks * ranks > sms) return rec_launch<T, VEC, COPY, GRAD, GATED, true, true>(g, maps, (unsigned)blocks, ranks);
+  return rec_launch<T, VEC, COPY, GRAD, GATED, true, false>(g, maps, (unsigned)blocks, ranks);
 }
 
 // Whether every operand can be moved in pieces of `bytes` (e: element size).

@@ -115,3 +115,52 @@ def test_embedding_grad_many_tokens_large_table(cp):
                      .astype(np.float16), 50257)
     check_table_grad(cp, np.resize(np.arange(0, 400009, 32), 70000), rng.standard_normal((70000, 50), dtype=np.float32),
                      400009)
+
+
+# ------------------------------------------------------------------ threads
+
+def test_threads_with_launches_of_different_sizes(cp):
+    """Calls from several threads at once whose launches of one kernel need
+    different amounts of shared memory (steps below, at and above the spans of
+    a block and of its ring; tokens of one to eight keys a thread)."""
+    import threading
+
+    from macmetalpy_b200 import _cuda_backend as cb
+
+    rng = np.random.default_rng(9)
+    work = []
+    for steps, tokens in ((40, 2000), (200, 20000), (3000, 60000), (90, 9000)):
+        a = rng.normal(2, 2, (2, steps, 96)).astype(np.float32)
+        work.append((a, rng.standard_normal(a.shape, dtype=np.float32), rng.integers(0, 3000, tokens),
+                     rng.standard_normal((tokens, 24), dtype=np.float32)))
+
+    def one(w, to, times):
+        a, x, ids, g = w
+        cb.check(cb.lib.mmp_init(cb.CudaBackend().device))  # the device of a new thread
+        A, X, I, G = cp.array(a), cp.array(x), cp.array(ids), cp.array(g)
+        for _ in range(times):
+            h = cp.linear_recurrence(A, X, gated=True)
+            da, dx, _ = cp.linear_recurrence_grad(A, X, h, X, gated=True)
+            to.append([r.get() for r in (h, da, dx, cp.embedding_grad(I, G, 3000))])
+
+    alone, together, failed = [[] for _ in work], [[] for _ in work], []
+
+    def guarded(w, to):
+        try:
+            one(w, to, 40)
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+
+    for w, to in zip(work, alone):
+        one(w, to, 1)
+    threads = [threading.Thread(target=guarded, args=(w, to)) for w, to in zip(work, together)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+    for p, q in zip(alone, together):
+        assert len(q) == 40
+        for r in q:
+            for got, want in zip(r, p[0]):
+                np.testing.assert_array_equal(got, want)

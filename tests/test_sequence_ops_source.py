@@ -84,3 +84,14 @@ def test_chained_kernels_promise_nothing_of_their_inputs(path):
 
 def test_files_of_chained_kernels_are_found():
     assert {"mmp_embedding.cu", "mmp_norm.cu", "mmp_recurrence.cu"} <= {os.path.basename(p) for p in CHAINED}
+
+
+@pytest.mark.parametrize("path", [p for p in SOURCES if "cudaFuncSetAttribute" in open(p).read()], ids=os.path.basename)
+def test_limits_of_shared_memory_are_set_once(path):
+    """A kernel's limit of dynamic shared memory is set once per device: set
+    anew by every call, another thread's call could lower it between this
+    one's setting and its launch."""
+    lines = open(path).read().splitlines()
+    for i, line in enumerate(lines):
+        if "cudaFuncSetAttribute(" in line:
+            assert any(re.search(r"if \(!\w+\[dev\]", before) for before in lines[max(0, i - 5):i]), (i + 1, line)
