@@ -90,6 +90,19 @@ __global__ void __launch_bounds__(256) emb_kernel(const T *w, long long rows, Fa
   if (bad) atomicExch(err, 5);
 }
 
+// ---- ids alone, of a call that has no element to write.
+template <class I>
+__global__ void __launch_bounds__(256) emb_ids_kernel(const I *ids, unsigned n, long long rows, int *err) {
+  chain_wait();
+  chain_next();
+  bool bad = false;
+  for (unsigned i = blockIdx.x * 256u + threadIdx.x; i < n; i += gridDim.x * 256u) {
+    const long long id = (long long)ids[i];
+    bad |= id < 0 || id >= rows;
+  }
+  if (bad) atomicExch(err, 5);
+}
+
 // Zeros to `n` elements by one warp: 16-byte pieces, the ends element by
 // element.
 template <class T> __device__ __forceinline__ void emb_zero(T *p, long long n) {
@@ -744,6 +757,16 @@ int run_emb(const void *w, int64_t rows, int64_t width, int64_t w_stride, const 
   });
 }
 
+int emb_ids(int ids_dtype, const void *ids, int64_t n, int64_t rows) {
+  const int64_t most = (int64_t)mmp::sm_count() * 8, want = (n + 255) / 256;
+  const unsigned grid = (unsigned)(want < most ? want : most);
+  int *err = mmp::device_error_word();
+  if (ids_dtype == MMP_INT32)
+    return mmp::launch_after(mmpd::emb_ids_kernel<int>, grid, 256, 0, 1, (const int *)ids, (unsigned)n, rows, err);
+  return mmp::launch_after(mmpd::emb_ids_kernel<long long>, grid, 256, 0, 1, (const long long *)ids, (unsigned)n, rows,
+                           err);
+}
+
 // Device memory of one call, from the stream-ordered pool.
 struct EmbBuf {
   void *p = nullptr;
@@ -906,9 +929,10 @@ int mmp_embedding(int dtype, const void *weight, int64_t rows, int64_t width, in
                   const void *ids, int64_t n, double scale, void *out) {
   int rc = emb_check("embedding", dtype, ids_dtype, rows, width, n);
   if (rc) return rc;
-  if (n == 0 || width == 0) return MMP_OK;
-  if (!ids || !out || (rows && !weight)) return mmp::set_error(MMP_E_ARG, "embedding: null pointer");
+  if (n == 0) return MMP_OK;
+  if (!ids || (width && (!out || (rows && !weight)))) return mmp::set_error(MMP_E_ARG, "embedding: null pointer");
   if (!mmp::device_error_word()) return mmp::set_error(MMP_E_CUDA, "no CUDA device available");
+  if (width == 0) return emb_ids(ids_dtype, ids, n, rows);
   MMP_EMB_DISPATCH(run_emb, weight, rows, width, w_stride, ids, n, scale, out);
 }
 
@@ -916,9 +940,12 @@ int mmp_embedding_grad(int dtype, int ids_dtype, const void *ids, int64_t n, con
                        int64_t rows, int64_t width, double scale, int64_t padding_idx, void *grad_weight) {
   int rc = emb_check("embedding_grad", dtype, ids_dtype, rows, width, n);
   if (rc) return rc;
-  if (rows == 0 || width == 0) return MMP_OK;
-  if ((n && (!ids || !grad)) || !grad_weight) return mmp::set_error(MMP_E_ARG, "embedding_grad: null pointer");
+  const bool empty = rows == 0 || width == 0;
+  if (empty && n == 0) return MMP_OK;
+  if ((n && !ids) || (!empty && ((n && !grad) || !grad_weight)))
+    return mmp::set_error(MMP_E_ARG, "embedding_grad: null pointer");
   if (!mmp::device_error_word()) return mmp::set_error(MMP_E_CUDA, "no CUDA device available");
+  if (empty) return emb_ids(ids_dtype, ids, n, rows);
   MMP_EMB_DISPATCH(run_emb_grad, ids, n, grad, g_stride, rows, width, scale, padding_idx, grad_weight);
 }
 

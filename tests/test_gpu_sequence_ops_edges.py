@@ -117,6 +117,28 @@ def test_embedding_grad_many_tokens_large_table(cp):
                      400009)
 
 
+@pytest.mark.parametrize("idt", ["int32", "int64"])
+@pytest.mark.parametrize("n", [1, 3, 3000, 70000])
+def test_bad_ids_of_empty_tables_are_reported(cp, n, idt):
+    """Without a row every id is out of range, and without a column those that
+    are beyond the rows, although there is nothing to write."""
+    ids = cp.zeros((n,), dtype=idt)
+    calls = [(True, lambda: cp.embedding(cp.zeros((0, 4), dtype="float32"), ids)),
+             (True, lambda: cp.embedding_grad(ids, cp.ones((n, 4), dtype="float32"), 0)),
+             (True, lambda: cp.embedding(cp.zeros((0, 0), dtype="float32"), ids)),
+             (True, lambda: cp.embedding_grad(ids, cp.ones((n, 0), dtype="float32"), 0)),
+             (False, lambda: cp.embedding(cp.zeros((2, 0), dtype="float32"), ids)),
+             (False, lambda: cp.embedding_grad(ids, cp.ones((n, 0), dtype="float32"), 2)),
+             (True, lambda: cp.embedding(cp.zeros((2, 0), dtype="float32"), ids + 2)),
+             (True, lambda: cp.embedding_grad(ids - 1, cp.ones((n, 0), dtype="float32"), 2))]
+    for k, (bad, call) in enumerate(calls):
+        assert call().size in (0, 4 * n), k
+        if bad:
+            with pytest.raises(RuntimeError, match="5"):
+                cp.synchronize()
+        cp.synchronize()
+
+
 # ------------------------------------------------------------------ threads
 
 def test_threads_with_launches_of_different_sizes(cp):
