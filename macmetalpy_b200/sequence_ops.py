@@ -270,12 +270,12 @@ def linear_recurrence_grad(a, x, h, grad, h0=None, *, axis=-2, gated=False, grad
             raise ValueError(f"{what}: shapes {', '.join(str(q._shape) for q in ops)} of a, h, grad"
                              f"{'' if x is None else ', x'} differ")
     axis = _axis(axis, len(shape), what)
+    if not gated:  # nor has it a part in the dtype
+        x, ops = None, ops[:3]
     dt = a._dtype
     if any(o._dtype != dt for o in ops):
         dt = resolve_dtype(np.result_type(*[o._dtype for o in ops]))
     _floating(dt, what)
-    if not gated:
-        x = None
     sdt = _F64 if dt == _F64 else _F32
     outer, steps, inner = _split(shape, axis)
     sshape = shape[:axis] + shape[axis + 1:]

@@ -237,3 +237,30 @@ def test_c_entries_refuse():
     assert L.mmp_global_norm(1, one, ptr, None, size, 1.0, 9, P) == -2                        # half norm
     size[0] = -3
     assert L.mmp_global_norm(1, one, ptr, None, size, 1.0, 10, P) == -2
+
+
+class Recorder:
+    """The library's calls with their arguments; each returns 0."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.calls.append((name, args))
+            return 0
+        return call
+
+
+def test_recurrence_grad_without_gates_leaves_x_alone(monkeypatch):
+    """x is not read there, so its dtype has no part in the result's."""
+    lib = Recorder()
+    monkeypatch.setattr(so._cb, "lib", lib)
+    a, h, g = (arr((2, 5, 3)) for _ in range(3))
+    for x in (arr((2, 5, 3), "float64"), arr((2, 5, 3), "int32"), None):
+        da, dx, _ = so.linear_recurrence_grad(a, x, h, g)
+        assert da.dtype == dx.dtype == np.float32
+        so.linear_recurrence_grad(a, x, h, g, out=(arr((2, 5, 3)), arr((2, 5, 3))))
+    assert [c[1][0] for c in lib.calls] == [so.MMP_CODES[np.dtype("float32")]] * 6
+    with pytest.raises(ValueError, match="differ"):
+        so.linear_recurrence_grad(a, arr((2, 5, 4)), h, g)
