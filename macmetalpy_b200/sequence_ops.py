@@ -39,10 +39,12 @@ _I32, _I64 = np.dtype(np.int32), np.dtype(np.int64)
 def _arr(x, what: str) -> ndarray:
     if x.__class__ is ndarray:
         return x
-    if x.__class__.__name__ == "DistArray":
-        raise TypeError(f"{what}: block-distributed arrays are not supported")
-    from .creation import asarray
-    return asarray(x)
+    if x.__class__.__name__ != "DistArray":
+        from .creation import asarray
+        x = asarray(x)  # of host data on a multi-rank job, this too can be block-distributed
+        if x.__class__.__name__ != "DistArray":
+            return x
+    raise TypeError(f"{what}: block-distributed arrays are not supported")
 
 
 def _floating(dt, what: str):

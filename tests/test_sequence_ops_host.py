@@ -264,3 +264,19 @@ def test_recurrence_grad_without_gates_leaves_x_alone(monkeypatch):
     assert [c[1][0] for c in lib.calls] == [so.MMP_CODES[np.dtype("float32")]] * 6
     with pytest.raises(ValueError, match="differ"):
         so.linear_recurrence_grad(a, arr((2, 5, 4)), h, g)
+
+
+def test_host_data_that_would_be_distributed_is_refused(monkeypatch):
+    """Above the shard threshold of a multi-rank job asarray() of host data
+    gives a block-distributed array."""
+    from macmetalpy_b200 import creation
+
+    class DistArray:
+        pass
+    monkeypatch.setattr(creation, "asarray", lambda obj: DistArray())
+    with pytest.raises(TypeError, match="distributed"):
+        so.linear_recurrence(np.zeros((2, 5, 3)), np.zeros((2, 5, 3)))
+    with pytest.raises(TypeError, match="distributed"):
+        so.embedding(arr((4, 3)), [1, 2])
+    with pytest.raises(TypeError, match="distributed"):
+        so.global_norm([np.zeros(3)])
