@@ -158,6 +158,13 @@ __device__ __forceinline__ void norm_scale(const T *x, T *y, int n, S coef) {
   for (int i = done + threadIdx.x; i < n; i += kNormThreads) y[i] = Cvt<T, S>::f(Cvt<S, T>::f(x[i]) * coef);
 }
 
+// The same where float32 holds fewer bits of the coefficient, or none of it
+// (below 2^-126: huge arrays and a small limit).  A call of its own, so that
+// the usual one keeps its registers.
+__device__ __noinline__ void norm_scale_small(const float *x, float *y, int n, double coef) {
+  for (int i = threadIdx.x; i < n; i += kNormThreads) y[i] = (float)(x[i] * coef);
+}
+
 template <int N>
 __global__ void __launch_bounds__(kNormThreads, 4) norm_scale_kernel(const __grid_constant__ NormTable<N> t,
                                                                   const double *partial, int npartial, double max_norm,
@@ -170,12 +177,14 @@ __global__ void __launch_bounds__(kNormThreads, 4) norm_scale_kernel(const __gri
     else *(float *)norm_out = (float)norm;
   }
   const double coef = norm <= max_norm ? 1.0 : max_norm / norm;
+  const bool small = coef < 0x1p-126 && coef > 0.0;
   for (int c = t.chunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {  // what was read last lies in L2
     const NormEntry &e = norm_find(t, c);
     if (coef == 1.0 && e.x == e.y) continue;  // in place, nothing to scale
     const long long at = (long long)(c - e.first) * kNormChunk;
     const int n = (int)(e.n - at < kNormChunk ? e.n - at : kNormChunk);
     if (e.dtype == MMP_DT_FLOAT16) norm_scale((const __half *)e.x + at, (__half *)e.y + at, n, (float)coef);
+    else if (e.dtype == MMP_DT_FLOAT32 && small) norm_scale_small((const float *)e.x + at, (float *)e.y + at, n, coef);
     else if (e.dtype == MMP_DT_FLOAT32) norm_scale((const float *)e.x + at, (float *)e.y + at, n, (float)coef);
     else norm_scale((const double *)e.x + at, (double *)e.y + at, n, coef);
   }

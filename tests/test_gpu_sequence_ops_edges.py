@@ -139,6 +139,27 @@ def test_bad_ids_of_empty_tables_are_reported(cp, n, idt):
         cp.synchronize()
 
 
+# ------------------------------------------------------------------ clipping
+
+@pytest.mark.parametrize("limit", [1.0, 1e-3, 1e-7, 1e-10, 1e-30, 1e-44])
+def test_clip_by_a_coefficient_below_float32(cp, limit):
+    """Huge gradients and a small limit: the coefficient passes float32's range
+    (subnormal from 1e-38 on), the clipped arrays need not.  The norm's sum in
+    float64 is within 2^-50 of 4100 terms; its root, the quotient, the
+    coefficient's rounding to 32 bits and the product's: 2 u and the result's
+    rounding."""
+    rng = np.random.default_rng(6)
+    arrays = [(rng.uniform(-3e38, 3e38, 4099)).astype(np.float32), np.float32([1e38, -1e25, 1.0]),
+              np.float16([60000, -3, 1e-7])]
+    norm = np.sqrt(sum((a.astype(np.float64) ** 2).sum() for a in arrays))
+    A = [cp.array(a) for a in arrays]
+    for out in (None, A):
+        res, _ = cp.clip_by_global_norm(A, limit, out=out)
+        for r, a in zip(res, arrays):
+            want = a.astype(np.float64) * (limit / norm)
+            close(r.get(), want, 2 * UNIT["float32"] * np.abs(want), str(a.dtype))
+
+
 # ------------------------------------------------------------------ threads
 
 def test_threads_with_launches_of_different_sizes(cp):
