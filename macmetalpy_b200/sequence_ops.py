@@ -196,7 +196,7 @@ def linear_recurrence(a, x, h0=None, *, axis=-2, gated=False, out=None, state_ou
         for ...:
             h = cp.linear_recurrence(gate, x, s, gated=True, state_out=s)
 
-    Decays are multiplied over up to 900 steps in the state's dtype; where they are
+    Decays are multiplied over up to 112 steps in the state's dtype; where they are
     larger than 1 and that product overflows, the result does too, unless the
     state before those steps is zero.
 

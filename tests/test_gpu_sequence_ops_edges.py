@@ -15,6 +15,45 @@ def cp():
     return cp
 
 
+# ------------------------------------------------------------------ recurrence
+
+# (outer, steps, inner) for every way rows reach the kernel, in clusters and in
+# blocks alone: tensor copies, a lane's own copies, loads of two bytes (float16)
+WAYS = [("float32", (1, 3000, 256)), ("float32", (1, 3000, 33)), ("float16", (1, 3000, 128)), ("float16", (1, 3000, 34)),
+        ("float16", (1, 3000, 33)), ("float64", (1, 1500, 64)), ("float64", (1, 1500, 33)), ("float32", (230, 250, 32)),
+        ("float16", (230, 250, 64)), ("float16", (230, 250, 33)), ("float16", (230, 250, 62)), ("float64", (230, 250, 32))]
+
+
+@pytest.mark.parametrize("dt,shape", WAYS)
+@pytest.mark.parametrize("decay", [16.0, 1024.0, 2.0 ** 15])
+def test_recurrence_decays_past_the_range(cp, dt, shape, decay):
+    """Decays whose product overflows within a span of steps or over the spans of
+    a block (up to 112 steps, 56 for float64): a state of zero stays zero, from
+    either end, and what is finite step by step is finite.  All values are
+    exact: sums of powers of two, rounded to the arrays' dtype once."""
+    last = {16.0: 4, 1024.0: 2, 2.0 ** 15: 2}[decay]
+    if dt == "float64":
+        decay, last = decay ** 12, 1  # 2^48, 2^120, 2^180 a step
+    a = cp.full(shape, decay, dtype=dt)
+    x = np.zeros(shape, dt)
+    x[:, -last:, ::2] = 1
+    want = np.zeros(shape)
+    for k in range(last):
+        want[:, shape[1] - last + k, ::2] = sum(decay ** j for j in range(k + 1))
+    st = cp.empty((shape[0], shape[2]), dtype="float64" if dt == "float64" else "float32")
+    h = cp.linear_recurrence(a, cp.array(x), state_out=st)
+    np.testing.assert_array_equal(h.get(), want.astype(dt))
+    np.testing.assert_array_equal(st.get(), want[:, -1])
+    # backward: gradients of the first steps alone, seen from the last step on
+    back, grad = want[:, ::-1], np.ascontiguousarray(x[:, ::-1])
+    ones = np.ones(shape, dt)
+    da, dx, _ = cp.linear_recurrence_grad(a, None, cp.array(ones), cp.array(grad))
+    np.testing.assert_array_equal(dx.get(), back.astype(dt))
+    back = back.copy()
+    back[:, 0] = 0  # h before the first step is zero
+    np.testing.assert_array_equal(da.get(), back.astype(dt))
+
+
 # ------------------------------------------------------------------ embedding gradient
 
 def table_grad(ids, g, rows, scale):
