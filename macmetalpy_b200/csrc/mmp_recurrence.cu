@@ -59,10 +59,12 @@ template <> struct RecState<double> { typedef double type; };
 
 // f = sigmoid(z) and 1 - f from e = exp(-|z|) in (0, 1], so that neither
 // cancels and z = +-inf gives exactly 1 and 0 (e = 0): a gate of +inf keeps
-// the state as it is, one of -inf replaces it.  A NaN goes to both.  float16
-// gates take ex2.approx and rcp.approx (relative errors 2^-22.5 + |z| 2^-24 and
-// 2^-23, far below the gates' own rounding of 2^-11): the kernel issues some
-// 20 instructions an element, and expf and the division would add as many.
+// the state as it is, one of -inf replaces it.  A NaN goes to both.  Gates in
+// 32 bits take rcp.approx in the place of a division (relative error 2^-23
+// against 2^-24), those of float16 arrays ex2.approx besides (2^-22.5 + 1.2 |z|
+// 2^-24, of which |z| 2^-24 and the constant's part come from the argument; far
+// below the gates' own rounding of 2^-11): the kernel issues some 20
+// instructions an element, and expf and the division would add as many.
 __device__ __forceinline__ float rec_ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -54,6 +54,39 @@ def test_recurrence_decays_past_the_range(cp, dt, shape, decay):
     np.testing.assert_array_equal(da.get(), back.astype(dt))
 
 
+def grow_as_computed(a, gated):
+    """K of the recurrence's bound for float16 gates, from the instructions that
+    make them: exp(-|z|) by ex2.approx within 2^-22.5 (2.8 u), its argument
+    |z| log2(e) rounded once and by a constant rounded to 0.2 u (1.2 |z| u);
+    1 + e u; rcp.approx 2^-23 (2 u); e r u: below 7 + 1.2 |z|.  The product
+    (1 - f) x, the fma and the decays' product add u each, and a state passed
+    on through three such products: 16 + 1.2 |z|.  |z| counts up to 104
+    (exp(-104) is zero)."""
+    assert a.dtype == np.float16 and gated
+    return 16 + 1.2 * np.minimum(np.abs(a.astype(np.float64)), 104)
+
+
+@pytest.mark.parametrize("spread", [1.0, 6.0, 20.0])
+@pytest.mark.parametrize("shape", [(3, 1, 40), (2, 30, 33), (1, 700, 128), (2, 300, 66), (2, 130, 65), (230, 130, 64)])
+def test_recurrence_float16_gates(cp, monkeypatch, shape, spread):
+    import test_gpu_sequence_ops as base
+    monkeypatch.setattr(base, "grow", grow_as_computed)
+    rng = np.random.default_rng(int(spread) + shape[1])
+    a = rng.normal(0, spread, shape).astype(np.float16)
+    x, g = (rng.standard_normal(shape).astype(np.float16) for _ in "xg")
+    h0 = rng.standard_normal((shape[0], shape[2])).astype(np.float32)
+    hs, es, last, el = base.recurrence(a, x, h0, True)
+    st = cp.empty(h0.shape, dtype="float32")
+    h = cp.linear_recurrence(cp.array(a), cp.array(x), cp.array(h0), gated=True, state_out=st)
+    close(h.get(), hs, es * UNIT["float16"], "float16")
+    close(st.get(), last, el * UNIT["float16"], "float32")
+    da, dx, dh0, ea, ex, e0 = base.recurrence_grad(a, x, h.get(), g, h0, None, True)
+    got = cp.linear_recurrence_grad(cp.array(a), cp.array(x), h, cp.array(g), cp.array(h0), gated=True)
+    close(got[0].get(), da, ea * UNIT["float16"], "float16")
+    close(got[1].get(), dx, ex * UNIT["float16"], "float16")
+    close(got[2].get(), dh0, e0 * UNIT["float16"], "float32")
+
+
 # ------------------------------------------------------------------ embedding gradient
 
 def table_grad(ids, g, rows, scale):
