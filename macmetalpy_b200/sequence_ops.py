@@ -182,7 +182,11 @@ def linear_recurrence(a, x, h0=None, *, axis=-2, gated=False, out=None, state_ou
     ``gated=False``: ``f = a`` and ``u = x`` (``a = 1`` is ``cumsum``).
     ``gated=True``: ``a`` holds logits, ``f = sigmoid(a)`` and ``u = (1 - f) * x``;
     a logit of ``+inf`` (a padded step) keeps the state as it is, one of
-    ``-inf`` (the first step of the next sequence in a packed row) replaces it.
+    ``-inf`` (the first step of the next sequence in a packed row) replaces it,
+    both exactly, where ``x`` and the state are finite.  The products are made:
+    an infinity or NaN in a padded step's ``x`` (``where`` puts zeros there) or in
+    the state before a new sequence gives NaN, as ``0 * inf`` is, and what is NaN
+    stays so to the end of its row.
 
     ``a`` and ``x`` have one shape, ``(..., steps, ...)``; the default axis is that
     of ``(batch, steps, width)``.  Slices of one larger array are read in place.
@@ -198,7 +202,8 @@ def linear_recurrence(a, x, h0=None, *, axis=-2, gated=False, out=None, state_ou
 
     Decays are multiplied over up to 112 steps in the state's dtype; where they are
     larger than 1 and that product overflows, the result does too, unless the
-    state before those steps is zero.
+    state before those steps is zero; where it underflows to zero, an infinite
+    state before them becomes NaN.
 
     Returns ``h``, of the shape and dtype of ``a`` and ``x`` (promoted together);
     it is written to ``out`` if that is given (``out`` may be ``a`` or ``x``).

@@ -87,6 +87,58 @@ def test_recurrence_float16_gates(cp, monkeypatch, shape, spread):
     close(got[2].get(), dh0, e0 * UNIT["float16"], "float32")
 
 
+MASKED = WAYS + [("float32", (3, 5, 40)), ("float16", (3, 14, 33)), ("float16", (3, 16, 64)), ("float64", (2, 9, 7)),
+                 ("float32", (2, 300, 96)), ("float16", (1, 9000, 64)), ("float32", (100, 400, 64))]
+
+
+def masked_inputs(dt, shape, seed):
+    """Gates of ordinary sequences, about one step in nine padded (+inf or the
+    type's highest value), and every 70 steps or so a new sequence (-inf or the
+    type's lowest value)."""
+    rng = np.random.default_rng(seed)
+    big = np.finfo(dt).max
+    z = rng.normal(0, 2, shape).astype(dt)
+    steps = shape[1]
+    pad, new = np.zeros(steps, bool), np.zeros(steps, bool)
+    pad[rng.random(steps) < 0.11] = True
+    new[rng.random(steps) < 0.014] = True
+    new[steps // 2], pad[0], pad[-1] = True, True, steps > 9
+    pad[new] = False
+    z[:, pad], z[:, new] = np.inf, -np.inf
+    z[:, pad, ::3], z[:, new, ::3] = big, -big
+    sdt = "float64" if dt == "float64" else "float32"
+    return (rng, z, rng.standard_normal(shape).astype(dt), rng.standard_normal((shape[0], shape[2])).astype(sdt),
+            rng.standard_normal(shape).astype(dt), pad, new, sdt)
+
+
+@pytest.mark.parametrize("dt,shape", MASKED)
+def test_recurrence_not_finite_to_the_end_of_its_chain(cp, dt, shape):
+    """An infinity or NaN in x, in a padded step too, or in the first state:
+    nothing finite comes after it in its chain, through padded steps and new
+    sequences (0 * inf is NaN); before it, and in other chains, every bit is
+    as it was."""
+    rng, z, x, h0, g, pad, new, sdt = masked_inputs(dt, shape, 1)
+
+    def run(x, h0):
+        st = cp.empty(h0.shape, dtype=sdt)
+        h = cp.linear_recurrence(cp.array(z), cp.array(x), cp.array(h0), gated=True, state_out=st)
+        return h.get(), st.get()
+    clean, last = run(x, h0)
+    assert np.isfinite(clean).all() and np.isfinite(last).all()
+    bad, bh0, want = x.copy(), h0.copy(), np.zeros(shape, bool)
+    at = {1: shape[1] // 3, 2: shape[1] - 1, 3: 0, 4: int(np.flatnonzero(pad)[-1])}
+    for k, v in ((1, np.inf), (2, np.nan), (3, -np.inf), (4, np.nan)):
+        bad[:, at[k], k::7] = v
+        want[:, at[k]:, k::7] = True
+    bh0[:, 5::7] = np.inf
+    want[:, :, 5::7] = True
+    h, st = run(bad, bh0)
+    np.testing.assert_array_equal(~np.isfinite(h), want)
+    np.testing.assert_array_equal(~np.isfinite(st), want[:, -1])
+    np.testing.assert_array_equal(h[~want], clean[~want])
+    np.testing.assert_array_equal(st[~want[:, -1]], last[~want[:, -1]])
+
+
 # ------------------------------------------------------------------ embedding gradient
 
 def table_grad(ids, g, rows, scale):
