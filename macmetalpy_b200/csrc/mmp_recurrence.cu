@@ -187,10 +187,13 @@ enum { kPlain, kLane, kTma };
 
 // Steps of one warp's span, by the bytes that a lane moves a step: 28 KB of
 // ring a stage and block of 7 warps, so that two blocks of three stages fit
-// an SM; kLane has half of that, which leaves its lines more of L1 (1 x 65521 x
-// 1001 float32 191 us, 226 with whole stages).
+// an SM.  kLane has half of that backward, which leaves its lines more of L1 (8
+// x 2048 x 2050 float16 gated 105 us, 113 with whole spans; 8 x 2048 x 1025
+// float32 plain 78, 81).  Forward it has whole spans (1 x 65521 x 1001 float32
+// 252 us, 306 with half ones; 8 x 2048 x 2050 float16 plain 53, 65, gated 61,
+// 59).
 template <int BYTES, int COPY, bool GRAD> struct RecSpan {
-  static constexpr int value = (GRAD ? 8 : 16) / (BYTES == 8 ? 2 : 1) / (COPY == kLane ? 2 : 1);
+  static constexpr int value = (GRAD ? 8 : 16) / (BYTES == 8 ? 2 : 1) / (COPY == kLane && GRAD ? 2 : 1);
 };
 
 template <class S> struct alignas(2 * sizeof(S)) RecMap {
