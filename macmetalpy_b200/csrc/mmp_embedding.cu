@@ -862,19 +862,22 @@ int run_emb_grad(const void *ids_, int64_t n, const void *grad_, int64_t g_strid
   EmbSorted e;
   e.n = (unsigned)n;
   e.sh = emb_shares(e.n, width, vec);
-  // keys, order (a second time each for sort_pairs), parts, list, bitmap, count
+  // keys, order (a second time each for sort_pairs), parts, list, then what
+  // sort_pairs wants zeroed with them: its state, bitmap, count
   const bool cluster = n <= mmpd::kEmbCluster;
   e.zeros = mmp::emb_zero_plan(rows, width * (int64_t)sizeof(T), cluster);
   const size_t np = ((size_t)n + 7) & ~(size_t)7, words = ((size_t)rows + 31) / 32;
   const size_t parts = (size_t)e.sh.shares * 2 * width * sizeof(typename mmpd::EmbAcc<T>::type);
   const size_t sorted = np * (cluster ? 8 : 16), lists = ((size_t)e.sh.shares * sizeof(mmpd::EmbRun) + 15) / 16 * 16;
-  int rc = mem.alloc(sorted + (parts + 15) / 16 * 16 + lists + words * 4 + 16);
+  const size_t state = cluster ? 0 : mmp::sort_pairs_state((unsigned)n, bits);
+  int rc = mem.alloc(sorted + (parts + 15) / 16 * 16 + lists + state + words * 4 + 16);
   if (rc) return rc;
   e.keys = (unsigned *)mem.p;
   e.order = e.keys + np;
   e.part = (char *)mem.p + sorted;
   e.list = (mmpd::EmbRun *)((char *)e.part + (parts + 15) / 16 * 16);
-  e.seen = (unsigned *)((char *)e.list + lists);
+  char *const zeroed = (char *)e.list + lists;
+  e.seen = (unsigned *)(zeroed + state);
   e.runs = e.seen + words;
   if (cluster) {
     const int items = (int)((n + mmpd::kSortThreads * mmpd::kSortRanks - 1) / (mmpd::kSortThreads * mmpd::kSortRanks));
@@ -900,12 +903,12 @@ int run_emb_grad(const void *ids_, int64_t n, const void *grad_, int64_t g_strid
     if (rc) return rc;
   } else {
     unsigned *const kb[2] = {e.keys, e.keys + 2 * np}, *const ob[2] = {e.order, e.order + 2 * np};
-    MMP_CUDA_TRY(cudaMemsetAsync(e.seen, 0, words * 4 + 4, mmp::stream()));
+    MMP_CUDA_TRY(cudaMemsetAsync(zeroed, 0, state + words * 4 + 4, mmp::stream()));
     mmpd::emb_prep_kernel<I><<<mmp::sm_count() * 2, 256, 0, mmp::stream()>>>(ids, (unsigned)n, rows, padding, kb[0],
                                                                              ob[0], e.seen, err);
     MMP_LAUNCH_CHECK("embedding_grad keys");
     int cur = 0;
-    rc = mmp::sort_pairs(kb, ob, (unsigned)n, bits, &cur);
+    rc = mmp::sort_pairs(kb, ob, (unsigned)n, bits, zeroed, &cur);
     if (rc) return rc;
     e.keys = kb[cur];
     e.order = ob[cur];

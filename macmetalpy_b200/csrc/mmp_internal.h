@@ -37,8 +37,18 @@ int scan_carry_allranks(int prod, int dtype, const void *agg, long long ntiles, 
                         void *carry_out);
 
 // Stable asynchronous sort of n keys below 2^bits with their payload between
-// two buffers each; *cur: the one that holds the result (mmp_sort.cu).
-int sort_pairs(unsigned *const keys[2], unsigned *const payload[2], unsigned n, int bits, int *cur);
+// two buffers each; *cur: the one that holds the result; `state`:
+// sort_pairs_state(n, bits) bytes aligned to 16, zeroed in the stream
+// (mmp_sort.cu).
+size_t sort_pairs_state(unsigned n, int bits);
+int sort_pairs(unsigned *const keys[2], unsigned *const payload[2], unsigned n, int bits, void *state, int *cur);
+// Inclusive sums of n > 0 counts, with its state in the caller's memory
+// (scan_counts_state(n) bytes, aligned to 16, zeroed in the stream;
+// mmp_scan.cu).  mmp_scan keeps its state from call to call and tells launches
+// apart by a number the host counts up, which a captured launch would repeat;
+// this may be captured and replayed.
+size_t scan_counts_state(long long n);
+int scan_counts(const unsigned *x, unsigned long long *y, long long n, void *state);
 
 }  // namespace mmp
 

@@ -238,6 +238,25 @@ struct ScanRun {
   }
 };
 
+// The look-back state of scan_counts: descriptors, then the tile counter.
+size_t scan_counts_state(long long n) { return (size_t)((n + STILE - 1) / STILE) * 16 + 256; }
+
+int scan_counts(const unsigned *x, unsigned long long *y, long long n, void *state) {
+  typedef ScanTypes<unsigned>::carry_t C;
+  static_assert(sizeof(TileDesc<C>) == 16, "scan_counts_state");
+  cudaStream_t st = stream();
+  int rc = set_stage_smem<unsigned, unsigned long long, false>();
+  if (rc) return rc;
+  const long long tiles = (n + STILE - 1) / STILE;
+  TileState<C> ts;
+  ts.desc = (TileDesc<C> *)state;
+  const int vec_ok = ((uintptr_t)x % 16 == 0) && ((uintptr_t)y % 16 == 0) && (n % 16 == 0);
+  scan_tiles_kernel<unsigned, unsigned long long, false><<<(unsigned)tiles, SBLOCK, StageSize<unsigned, unsigned long long>(), st>>>(
+      x, y, 1, n, tiles, tiles, ts, (unsigned *)((char *)state + tiles * 16), 1u, device_error_word(), nullptr, vec_ok);
+  MMP_LAUNCH_CHECK("scan_tiles_kernel (counts)");
+  return MMP_OK;
+}
+
 }  // namespace mmp
 
 extern "C" int mmp_scan(int op, int dtype, const void *x, int out_dtype, void *y, int64_t outer, int64_t k,

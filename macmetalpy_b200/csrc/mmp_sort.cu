@@ -476,13 +476,19 @@ int run_passes(const T *x, T *y, long long *idx, unsigned long long rows, unsign
 
 }  // namespace
 
+// Digit counts of one pass of sort_pairs.
+static size_t sort_counts(unsigned n) { return ((size_t)n + RS_TILE - 1) / RS_TILE * 256; }
+
+size_t sort_pairs_state(unsigned n, int bits) { return scan_counts_state((long long)sort_counts(n)) * ((bits + 7) / 8); }
+
 // Stable sort of n 32-bit keys below 2^bits with a 32-bit payload, between
 // two buffers each (keys[0], payload[0] hold the input); *cur is where the
-// result lies.  Asynchronous: no pass is skipped (mmp_internal.h).
-int sort_pairs(unsigned *const keys[2], unsigned *const payload[2], unsigned n, int bits, int *cur) {
+// result lies.  Asynchronous: no pass is skipped, and nothing is kept between
+// calls, so it may be captured (mmp_internal.h).
+int sort_pairs(unsigned *const keys[2], unsigned *const payload[2], unsigned n, int bits, void *state, int *cur) {
   cudaStream_t st = stream();
-  const unsigned tiles = (unsigned)(((unsigned long long)n + RS_TILE - 1) / RS_TILE);
-  const size_t nc = (size_t)tiles * 256;
+  const size_t nc = sort_counts(n), each = scan_counts_state((long long)nc);
+  const unsigned tiles = (unsigned)(nc / 256);
   PoolBuf cnt, inc;
   int rc = cnt.alloc(nc * 4);
   if (!rc) rc = inc.alloc(nc * 8);
@@ -491,7 +497,7 @@ int sort_pairs(unsigned *const keys[2], unsigned *const payload[2], unsigned n, 
   for (int shift = 0; shift < bits; shift += 8, *cur ^= 1) {
     rs_hist<unsigned, false><<<tiles, RS_THREADS, 0, st>>>(keys[*cur], nullptr, n, shift, (unsigned *)cnt.p, tiles);
     MMP_LAUNCH_CHECK("rs_hist");
-    rc = mmp_scan(MMP_S_SUM, MMP_UINT32, cnt.p, MMP_UINT64, inc.p, 1, (int64_t)nc, 1, nullptr);
+    rc = scan_counts((const unsigned *)cnt.p, (unsigned long long *)inc.p, (long long)nc, (char *)state + each * (shift / 8));
     if (rc) return rc;
     rc = launch_scatter<unsigned, true, false, false>(keys[*cur], keys[*cur ^ 1], payload[*cur], payload[*cur ^ 1], nullptr,
                                                       nullptr, n, shift, (const unsigned *)cnt.p,

@@ -331,3 +331,66 @@ def test_threads_with_launches_of_different_sizes(cp):
         for r in q:
             for got, want in zip(r, p[0]):
                 np.testing.assert_array_equal(got, want)
+
+
+# ------------------------------------------------------------------ captured
+
+CAPTURE = """
+import sys
+sys.path.insert(0, {repo!r})
+import ctypes
+import numpy as np
+import torch
+import macmetalpy_b200 as cp
+from macmetalpy_b200 import _cuda_backend as cb
+cp.synchronize()
+stream = torch.cuda.Stream()
+cb.check(cb.lib.mmp_set_stream(ctypes.c_void_p(stream.cuda_stream)))
+rng = np.random.default_rng(0)
+n, width = 70000, 6
+tables = [200, 5000, 50257 * 30]
+ids = [cp.array(rng.integers(0, rows, n)) for rows in tables]
+g = cp.array(rng.standard_normal((n, width)).astype("float32"))
+out = [cp.empty((rows, width), dtype="float32") for rows in tables]
+def step():
+    for i, rows, o in zip(ids, tables, out):
+        cp.embedding_grad(i, g, rows, 2.0, out=o)
+def results():
+    return [o.get() for o in out]
+graphs = []
+for _ in range(2):  # the first calls of this process: nothing is set up before the capture
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        step()
+    graphs.append(graph)
+for k in range(6):
+    for i, rows in zip(ids, tables):
+        i.set(rng.integers(0, rows, n))
+    g.set(rng.standard_normal((n, width)).astype("float32"))
+    cp.cumsum(cp.ones(((k + 1) << 22,), dtype="float32"))  # grows and moves the library's own scan state
+    step(); want = results()
+    for o in out:
+        o.fill(7)
+    cp.synchronize()
+    for _ in range(1 + k % 2):
+        with torch.cuda.stream(stream):
+            graphs[k % 2].replay()
+    torch.cuda.synchronize()
+    for p, q in zip(want, results()):
+        np.testing.assert_array_equal(p, q)
+    cp.synchronize()
+print("captured")
+"""
+
+
+def test_many_tokens_captured_and_replayed(cp):
+    """The gradient above 65536 tokens in two graphs, replayed in turn and twice
+    in a row, sort keys of one pass and of several, other scans in between (a
+    process of its own: the library keeps the stream it is given)."""
+    import os
+    import subprocess
+    import sys
+
+    repo = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    p = subprocess.run([sys.executable, "-c", CAPTURE.format(repo=repo)], capture_output=True, text=True, timeout=300)
+    assert p.returncode == 0 and "captured" in p.stdout, p.stdout + p.stderr

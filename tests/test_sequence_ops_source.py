@@ -95,3 +95,19 @@ def test_limits_of_shared_memory_are_set_once(path):
     for i, line in enumerate(lines):
         if "cudaFuncSetAttribute(" in line:
             assert any(re.search(r"if \(!\w+\[dev\]", before) for before in lines[max(0, i - 5):i]), (i + 1, line)
+
+
+def test_the_embedding_gradients_sort_keeps_nothing_between_calls():
+    """mmp_scan keeps look-back state of the device from call to call, told
+    apart by a number that the host counts up and a captured launch repeats:
+    sort_pairs brings its own, zeroed in the stream."""
+    text = open(os.path.join(REPO, "macmetalpy_b200", "csrc", "mmp_sort.cu")).read()
+    body = text[text.index("int sort_pairs("):]
+    body = body[:body.index("\n}\n")]
+    assert "mmp_scan(" not in body and "scratch(" not in body
+    scan = open(os.path.join(REPO, "macmetalpy_b200", "csrc", "mmp_scan.cu")).read()
+    body = scan[scan.index("int scan_counts("):]
+    body = body[:body.index("\n}\n")]
+    assert "scan_state(" not in body
+    grad = open(os.path.join(REPO, "macmetalpy_b200", "csrc", "mmp_embedding.cu")).read()
+    assert "cudaMemsetAsync(zeroed, 0, state +" in grad
