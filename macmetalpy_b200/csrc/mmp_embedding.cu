@@ -23,9 +23,10 @@
 // not marked __restrict__: a kernel launched by launch_after is resident while
 // the one before it still writes them, and a load that passes for one of
 // constant memory need not stay behind chain_wait.
-// Whole calls: lookup of 16384 x 1024 float32 18 us (writes alone take 17 at
-// the fill rate); gradient of 512 tokens, 8192 x 768 float32 10 us, of 16384
-// tokens, 50257 x 2048 float16 70 us (fill rate 52, copy rate 42).
+// Whole calls: lookup of 16384 of 128000 x 1024 float32 17 us (writes alone take
+// 17 at the fill rate); gradient of 512 tokens, 8192 x 768 float32 8.4 us, of
+// 16384 tokens, 50257 x 2048 float16 69 us (fill rate 52, copy rate 42), of
+// 131072 tokens, 50257 x 768 float16 145 us.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

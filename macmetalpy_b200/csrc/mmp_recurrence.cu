@@ -30,7 +30,8 @@
 // next spans into a ring in shared memory that only it reads.
 // Whole calls: 1 x 65521 x 1000 float32 121 to 131 us (6.0 to 6.5 TB/s); 8 x
 // 2048 x 2048 float16 gated 44 us (4.6 TB/s; latency, and 256 blocks on 148
-// SMs), its gradient 76 (5.3); 2 x 16383 x 1536 float32 gradient 176 (5.7).
+// SMs), its gradient 75 to 80 (5.0 to 5.4); 2 x 16383 x 1536 float32 gradient
+// 172 to 180 (5.6 to 5.9).
 #include <cooperative_groups.h>
 #include <cuda.h>
 #include <cuda_fp16.h>

@@ -538,8 +538,9 @@ def global_norm(arrays, *, out=None):
     """Euclidean norm over all elements of a list of arrays, as one 0-d array.
 
     ``sqrt(sum(sum(x * x) for x in arrays))`` for arrays of any shapes and
-    floating dtypes, summed in float64; float32, or float64 if one of the
-    arrays is.  An empty list has norm 0.
+    floating dtypes, summed in float64 (where squares of float64 elements
+    beyond 1e154 are infinite); float32, or float64 if one of the arrays is.
+    An empty list has norm 0.
     """
     what = "global_norm"
     return _norm_call(_norm_list(arrays, what), None, 0.0, out, what, "out")
